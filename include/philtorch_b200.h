@@ -41,7 +41,8 @@ typedef void* ptb_stream_t; /* a cudaStream_t */
 
 enum { PTB_F32 = 0, PTB_F64 = 1,
        PTB_C64 = 2, PTB_C128 = 3, /* interleaved {re, im}; first-order recurrences only */
-       PTB_F16 = 4, PTB_BF16 = 5  /* 2-byte arrays, float32 arithmetic; first-order recurrences only */ };
+       PTB_F16 = 4, PTB_BF16 = 5  /* 2-byte arrays, float32 arithmetic; first-order recurrences,
+                                         linear attention, layer norm */ };
 enum {
   PTB_OK = 0,
   PTB_ERR_ARG = 1,       /* null pointer, negative size, unknown dtype */
@@ -492,6 +493,54 @@ int ptb_modal_bank_bwd(int dtype, int64_t rows, int64_t M, int64_t N, const void
                        const void* gain, const void* coef, const void* d, const void* fwd_chk, const void* gy,
                        const void* g_wf, int need, void* grad_x, void* grad_w0, void* partial, void* chk,
                        ptb_stream_t stream);
+
+/* ---- linear attention with decays ------------------------------------------------------------
+ * The first-order recurrence on a matrix state: S[t] = exp(g[t]) S[t-1] + k[t] v[t]^T, o[t] = scale q[t]^T S[t].
+ * dtype: PTB_F32, PTB_F64, PTB_F16 or PTB_BF16 for q, k, v, o and their gradients; log_decay, the states and their
+ * gradients hold float64 beside PTB_F64, else float32.  q, k: (B,T,H,Dk), v: (B,T,H,Dv), 1 <= Dk, Dv <= 128, the last
+ * axis dense; *_strides: three element strides (batch, time, head), zero where an axis is shared.  log_decay likewise
+ * (batch and time stride zero: one decay per head); -inf is a decay of zero.  lengths: optional (B,), clamped to
+ * 0..T: tokens from lengths[b] on are not read, leave the state alone and give zeros.  init, fin: optional dense
+ * (B,H,Dk,Dv), the state before the first and after the last token.  o: dense (B,T,H,Dv).
+ * workspace: ptb_linear_attention_workspace_bytes(..., backward, decay_grad) bytes, 256-byte aligned, private to the
+ * call until it completes.  status is not used (no kernel here waits on another CTA); it may be NULL. */
+int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
+                                             int backward, int decay_grad);
+int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                             const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                             const int32_t* lengths, const void* init, double scale, void* o, void* fin,
+                             void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream);
+/* Adjoint: the gradients of q, k, v (dense, shaped like them), of the log decays ((B,T,H) when
+ * grad_log_decay_per_token, else (H)) and of the initial state, each optional.  grad_fin: optional gradient of fin.
+ * The states are recomputed; nothing of the forward call has to be kept. */
+int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                             const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                             const int32_t* lengths, const void* init, double scale, const void* grad_o,
+                             const int64_t* grad_o_strides, const void* grad_fin, void* grad_q, void* grad_k,
+                             void* grad_v, void* grad_log_decay, int grad_log_decay_per_token, void* grad_init,
+                             void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream);
+/* One token of every sequence: state (B,H,Dk,Dv) is updated in place (its matrices dense, state_strides: two element
+ * strides (batch, head)); q, k: (B,H,Dk), v: (B,H,Dv) and log_decay with two strides each; o: dense (B,H,Dv). */
+int ptb_linear_attention_step(int dtype, int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                              double scale, void* state, const int64_t* state_strides, void* o, ptb_stream_t stream);
+
+/* ---- layer norm over groups of channels --------------------------------------------------------
+ * x: rows of groups * width channels (dense), x_stride elements apart; y dense.  weight, bias: optional
+ * (groups * width), of the storage type, or float32 / float64 when params_wide.  mean, rstd: (rows, groups) in float32
+ * (float64 beside PTB_F64), written by the forward call (both optional there) and read by the adjoint.
+ * 1 <= width <= 16384, groups <= 65535.  The parameter gradients have the parameters' type. */
+int64_t ptb_layer_norm_bwd_workspace_bytes(int dtype, int64_t rows, int64_t groups, int64_t width);
+int ptb_layer_norm_fwd(int dtype, int64_t rows, int64_t groups, int64_t width, const void* x, int64_t x_stride,
+                       const void* weight, const void* bias, int params_wide, double eps, void* y, void* mean,
+                       void* rstd, ptb_stream_t stream);
+int ptb_layer_norm_bwd(int dtype, int64_t rows, int64_t groups, int64_t width, const void* x, int64_t x_stride,
+                       const void* weight, int params_wide, const void* mean, const void* rstd, const void* grad_y,
+                       int64_t grad_y_stride, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                       int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -156,6 +156,24 @@ lib.ptb_lpv_biquad_tdf2_fwd.restype = _i32
 lib.ptb_lpv_biquad_tdf2_bwd.argtypes = lib.ptb_lpv_biquad_df2_bwd.argtypes
 lib.ptb_lpv_biquad_tdf2_bwd.restype = _i32
 
+_strides = ctypes.POINTER(_i64)
+_la_in = [_i32] + [_i64] * 5 + [_vp, _strides] * 4 + [_vp, _vp, ctypes.c_double]
+lib.ptb_linear_attention_workspace_bytes.argtypes = [_i32] + [_i64] * 5 + [_i32, _i32]
+lib.ptb_linear_attention_workspace_bytes.restype = _i64
+lib.ptb_linear_attention_fwd.argtypes = _la_in + [_vp, _vp] + _tail
+lib.ptb_linear_attention_fwd.restype = _i32
+lib.ptb_linear_attention_bwd.argtypes = _la_in + [_vp, _strides] + [_vp] * 5 + [_i32, _vp] + _tail
+lib.ptb_linear_attention_bwd.restype = _i32
+lib.ptb_linear_attention_step.argtypes = ([_i32] + [_i64] * 4 + [_vp, _strides] * 4 + [ctypes.c_double, _vp, _strides, _vp]
+                                          + [_vp])
+lib.ptb_linear_attention_step.restype = _i32
+lib.ptb_layer_norm_bwd_workspace_bytes.argtypes = [_i32] + [_i64] * 3
+lib.ptb_layer_norm_bwd_workspace_bytes.restype = _i64
+lib.ptb_layer_norm_fwd.argtypes = [_i32] + [_i64] * 3 + [_vp, _i64, _vp, _vp, _i32, ctypes.c_double] + [_vp] * 3 + [_vp]
+lib.ptb_layer_norm_fwd.restype = _i32
+lib.ptb_layer_norm_bwd.argtypes = ([_i32] + [_i64] * 3 + [_vp, _i64, _vp, _i32] + [_vp] * 3 + [_i64] + [_vp] * 3 + _tail)
+lib.ptb_layer_norm_bwd.restype = _i32
+
 _status: dict[int, torch.Tensor] = {}
 
 ERROR_BITS = {1: "look-back wait expired", 2: "tile load wait expired", 4: "tile drain wait expired",
@@ -242,6 +260,20 @@ def call(fn, device: torch.device, B: int, T: int, *args, ws_bytes: int = -1) ->
         check(rc, fn.__name__)
     if CHECK_EVERY_CALL:
         check_errors(device)
+
+
+def launch(fn, device: torch.device, *args) -> None:
+    """Runs ``fn(*args, stream)``, an entry point without workspace and waits, on ``device``'s current stream."""
+    idx = device.index
+    if idx is None:
+        idx = _current_device()
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            rc = fn(*args, _current_raw_stream(idx))
+    else:
+        rc = fn(*args, _current_raw_stream(idx))
+    if rc != 0:
+        check(rc, fn.__name__)
 
 
 # PHILTORCH_B200_CHECK=1: every call synchronises and raises at once if a device-side wait expired

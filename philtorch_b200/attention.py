@@ -1,0 +1,291 @@
+"""Linear attention with a decay for each head: the recurrences of this package on a matrix state,
+
+    S[t] = exp(g[t]) S[t-1] + k[t] v[t]^T,      o[t] = scale * q[t]^T S[t]
+
+``lti.linear_attention`` (one decay per head) and ``lpv.linear_attention`` (one per token and head) are
+thin front ends of this module, like ``linear_recurrence`` and ``state_space`` beside them: torch custom ops
+(``torch.ops.philtorch_b200.linear_attention*``), an autograd Function with fused adjoint kernels, and the
+argument checks.  The coefficient with time index t multiplies the PREVIOUS state, as everywhere in
+this package; it is passed as its logarithm, so that decays near one keep their precision and a decay of
+zero (``-inf``: the sequence starts anew at this token) is an ordinary value.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Any, Optional, Tuple
+
+import torch
+from torch import Tensor
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import lib, ptr
+from .norm import layer_norm
+from .ops import _LIB, _TAGS
+
+__all__ = ["LinearAttention", "MAX_HEAD_DIM"]
+
+MAX_HEAD_DIM = 128
+_CODES = {torch.float32: _lib.PTB_F32, torch.float64: _lib.PTB_F64, torch.float16: _lib.PTB_F16,
+          torch.bfloat16: _lib.PTB_BF16}
+_I3, _I2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
+
+
+def state_dtype(dtype: torch.dtype) -> torch.dtype:
+    """Type of the states and of the log decays: float64 beside float64 tensors, else float32."""
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def _rows(t: Tensor) -> Tensor:
+    """The tensor with its last axis dense; the other strides are the kernels' arguments (views of one fused
+    projection, or heads shared through ``expand``, are read in place)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _code(t: Tensor) -> int:
+    try:
+        return _CODES[t.dtype]
+    except KeyError:
+        raise RuntimeError("linear attention takes float32, float64, float16 and bfloat16 tensors, "
+                           f"got {t.dtype}") from None
+
+
+def _check(q: Tensor, k: Tensor, v: Tensor, g: Tensor, init: Optional[Tensor], lengths: Optional[Tensor]) -> None:
+    torch._check(q.dim() == 4, lambda: f"q must be 4D (batch, time, heads, Dk), got {tuple(q.shape)}")
+    torch._check(k.shape == q.shape, lambda: f"k must have the shape of q, got {tuple(k.shape)} and {tuple(q.shape)}")
+    torch._check(v.dim() == 4 and v.shape[:3] == q.shape[:3],
+                 lambda: f"v must be (batch, time, heads, Dv) beside q {tuple(q.shape)}, got {tuple(v.shape)}")
+    B, T, H, Dk = q.shape
+    Dv = v.shape[3]
+    torch._check(1 <= Dk <= MAX_HEAD_DIM and 1 <= Dv <= MAX_HEAD_DIM,
+                 lambda: f"head sizes Dk = {Dk}, Dv = {Dv}: the kernels cover 1..{MAX_HEAD_DIM}.")
+    torch._check(k.dtype == q.dtype and v.dtype == q.dtype,
+                 lambda: f"q, k and v must have the same type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    wide = state_dtype(q.dtype)
+    torch._check(g.dtype == wide, lambda: f"log_decay must be {wide} beside {q.dtype} tensors, got {g.dtype}")
+    torch._check(tuple(g.shape) in ((H,), (B, T, H)),
+                 lambda: f"log_decay must be (heads,) or (batch, time, heads), got {tuple(g.shape)}")
+    if init is not None:
+        torch._check(tuple(init.shape) == (B, H, Dk, Dv),
+                     lambda: f"the initial state must be {(B, H, Dk, Dv)}, got {tuple(init.shape)}")
+        torch._check(init.dtype == wide, lambda: f"the initial state must be {wide} beside {q.dtype} tensors, got {init.dtype}")
+    if lengths is not None:
+        torch._check(tuple(lengths.shape) == (B,), lambda: f"lengths must be ({B},), got {tuple(lengths.shape)}")
+        torch._check(lengths.dtype in (torch.int32, torch.int64), lambda: f"lengths must be int32 or int64, got {lengths.dtype}")
+        torch._check(T < 2 ** 31, lambda: "lengths are for fewer than 2^31 tokens")
+
+
+def _decay_strides(g: Tensor):
+    return _I3(0, 0, g.stride(0)) if g.dim() == 1 else _I3(*g.stride())
+
+
+def _strides(t: Tensor):
+    return _I3(*t.stride()[:3])
+
+
+_ws_bytes: dict = {}
+
+
+def _workspace_bytes(code: int, B: int, T: int, H: int, Dk: int, Dv: int, backward: int, decay: int) -> int:
+    key = (code, B, T, H, Dk, Dv, backward, decay)
+    n = _ws_bytes.get(key)
+    if n is None:
+        if len(_ws_bytes) > 4096:   # a server sees many lengths
+            _ws_bytes.clear()
+        n = _ws_bytes[key] = lib.ptb_linear_attention_workspace_bytes(code, B, T, H, Dk, Dv, backward, decay)
+    return n
+
+
+def _int_lengths(lengths: Optional[Tensor], T: int) -> Optional[Tensor]:
+    if lengths is None:
+        return None
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, T).to(torch.int32)
+    return lengths.contiguous()
+
+
+# ------------------------------------------------------------------------------------------------ ops
+_LIB.define("linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? init, Tensor? lengths, "
+            "float scale, bool want_state) -> (Tensor, Tensor)", tags=_TAGS)
+_LIB.define("linear_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? init, Tensor? lengths, "
+            "float scale, Tensor? grad_o, Tensor? grad_state, bool need_q, bool need_k, bool need_v, "
+            "bool need_decay, bool need_init) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", tags=_TAGS)
+_LIB.define("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, float scale) "
+            "-> Tensor", tags=_TAGS)
+
+
+def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state):
+    _check(q, k, v, log_decay, init, lengths)
+    dev = _lib.require_cuda(q, k, v, log_decay, init, lengths)
+    code = _code(q)
+    B, T, H, Dk = q.shape
+    Dv = v.shape[3]
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    init = None if init is None else init.contiguous()
+    lengths = _int_lengths(lengths, T)
+    o = v.new_empty((B, T, H, Dv))
+    state = log_decay.new_empty((B, H, Dk, Dv) if want_state else (0,))
+    if B and H and (T or want_state):
+        _lib.call(lib.ptb_linear_attention_fwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides(q), ptr(k), _strides(k),
+                  ptr(v), _strides(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(o),
+                  ptr(state) if want_state else None, ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 0, 0))
+    return o, state
+
+
+def _linear_attention_bwd(q, k, v, log_decay, init, lengths, scale, grad_o, grad_state, need_q, need_k, need_v,
+                          need_decay, need_init):
+    dev = _lib.require_cuda(q, k, v, log_decay, init, lengths, grad_o, grad_state)
+    code = _code(q)
+    B, T, H, Dk = q.shape
+    Dv = v.shape[3]
+    if grad_o is None:   # only the final state was used
+        grad_o = v.new_zeros(Dv).expand(B, T, H, Dv)
+    q, k, v, grad_o = _rows(q), _rows(k), _rows(v), _rows(grad_o)
+    init = None if init is None else init.contiguous()
+    grad_state = None if grad_state is None else grad_state.contiguous()
+    lengths = _int_lengths(lengths, T)
+    gq, gk, gv = (t.new_empty(t.shape if need else (0,)) for t, need in ((q, need_q), (k, need_k), (v, need_v)))
+    gg = log_decay.new_empty(log_decay.shape if need_decay else (0,))
+    ginit = log_decay.new_empty((B, H, Dk, Dv) if need_init else (0,))
+    if B and H:
+        opt = lambda t, need: ptr(t) if need else None   # noqa: E731
+        _lib.call(lib.ptb_linear_attention_bwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides(q), ptr(k), _strides(k),
+                  ptr(v), _strides(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(grad_o),
+                  _strides(grad_o), ptr(grad_state), opt(gq, need_q), opt(gk, need_k), opt(gv, need_v),
+                  opt(gg, need_decay), int(log_decay.dim() == 3), opt(ginit, need_init),
+                  ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 1, int(need_decay)))
+    else:
+        gg.zero_()
+    return gq, gk, gv, gg, ginit
+
+
+def _check_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, state: Tensor) -> None:
+    torch._check(q.dim() == 3, lambda: f"q must be 3D (batch, heads, Dk), got {tuple(q.shape)}")
+    torch._check(k.shape == q.shape, lambda: f"k must have the shape of q, got {tuple(k.shape)} and {tuple(q.shape)}")
+    torch._check(v.dim() == 3 and v.shape[:2] == q.shape[:2],
+                 lambda: f"v must be (batch, heads, Dv) beside q {tuple(q.shape)}, got {tuple(v.shape)}")
+    B, H, Dk = q.shape
+    Dv = v.shape[2]
+    torch._check(1 <= Dk <= MAX_HEAD_DIM and 1 <= Dv <= MAX_HEAD_DIM,
+                 lambda: f"head sizes Dk = {Dk}, Dv = {Dv}: the kernels cover 1..{MAX_HEAD_DIM}.")
+    torch._check(k.dtype == q.dtype and v.dtype == q.dtype,
+                 lambda: f"q, k and v must have the same type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    wide = state_dtype(q.dtype)
+    torch._check(g.dtype == wide, lambda: f"log_decay must be {wide} beside {q.dtype} tensors, got {g.dtype}")
+    torch._check(tuple(g.shape) in ((H,), (B, H)),
+                 lambda: f"log_decay must be (heads,) or (batch, heads), got {tuple(g.shape)}")
+    torch._check(tuple(state.shape) == (B, H, Dk, Dv), lambda: f"state must be {(B, H, Dk, Dv)}, got {tuple(state.shape)}")
+    torch._check(state.dtype == wide, lambda: f"state must be {wide} beside {q.dtype} tensors, got {state.dtype}")
+    # it is written in place: each (Dk, Dv) matrix dense, no two of them sharing memory
+    ok = (state.stride(3) == 1 or Dv == 1) and (state.stride(2) == Dv or Dk == 1)
+    room = Dk * Dv
+    for stride, size in sorted((state.stride(i), state.shape[i]) for i in (0, 1) if state.shape[i] > 1):
+        ok = ok and stride >= room
+        room = stride * size
+    torch._check(ok or state.numel() == 0, lambda: "state is updated in place: its (Dk, Dv) matrices must be dense and "
+                                                   f"apart from one another, got strides {tuple(state.stride())}")
+
+
+def _linear_attention_step(q, k, v, log_decay, state, scale):
+    _check_step(q, k, v, log_decay, state)
+    dev = _lib.require_cuda(q, k, v, log_decay, state)
+    B, H, Dk = q.shape
+    Dv = v.shape[2]
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    o = v.new_empty((B, H, Dv))
+    if B and H:
+        gs = _I2(0, log_decay.stride(0)) if log_decay.dim() == 1 else _I2(*log_decay.stride())
+        _lib.launch(lib.ptb_linear_attention_step, dev, _code(q), B, H, Dk, Dv, ptr(q), _I2(*q.stride()[:2]), ptr(k),
+                    _I2(*k.stride()[:2]), ptr(v), _I2(*v.stride()[:2]), ptr(log_decay), gs, scale, ptr(state),
+                    _I2(*state.stride()[:2]), ptr(o))
+        torch.autograd.graph.increment_version(state)
+    return o
+
+
+_LIB.impl("linear_attention", _linear_attention, "CUDA")
+_LIB.impl("linear_attention_bwd", _linear_attention_bwd, "CUDA")
+_LIB.impl("linear_attention_step", _linear_attention_step, "CUDA")
+
+
+@torch.library.register_fake("philtorch_b200::linear_attention")
+def _(q, k, v, log_decay, init, lengths, scale, want_state):
+    _check(q, k, v, log_decay, init, lengths)
+    B, T, H, Dk = q.shape
+    return v.new_empty((B, T, H, v.shape[3])), log_decay.new_empty((B, H, Dk, v.shape[3]) if want_state else (0,))
+
+
+@torch.library.register_fake("philtorch_b200::linear_attention_bwd")
+def _(q, k, v, log_decay, init, lengths, scale, grad_o, grad_state, need_q, need_k, need_v, need_decay, need_init):
+    gq, gk, gv = (t.new_empty(t.shape if need else (0,)) for t, need in ((q, need_q), (k, need_k), (v, need_v)))
+    B, T, H, Dk = q.shape
+    return (gq, gk, gv, log_decay.new_empty(log_decay.shape if need_decay else (0,)),
+            log_decay.new_empty((B, H, Dk, v.shape[3]) if need_init else (0,)))
+
+
+@torch.library.register_fake("philtorch_b200::linear_attention_step")
+def _(q, k, v, log_decay, state, scale):
+    _check_step(q, k, v, log_decay, state)
+    return v.new_empty(v.shape)
+
+
+_ops = torch.ops.philtorch_b200
+
+
+# ------------------------------------------------------------------------------------------------ autograd
+class LinearAttention(Function):
+    """(q, k, v, log_decay, init or None, lengths or None, scale, want_state) -> (o, final state).  First
+    derivatives; the backward pass recomputes the states instead of keeping them."""
+
+    @staticmethod
+    def forward(ctx: Any, q, k, v, log_decay, init, lengths, scale: float, want_state: bool):
+        o, state = _ops.linear_attention(q, k, v, log_decay, init, lengths, scale, want_state)
+        ctx.save_for_backward(q, k, v, log_decay, init, lengths)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        if not want_state:
+            ctx.mark_non_differentiable(state)
+        return o, state
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad_o: Optional[Tensor], grad_state: Optional[Tensor]):
+        need = ctx.needs_input_grad[:5]
+        if (grad_o is None and grad_state is None) or not any(need):
+            return (None,) * 8
+        q, k, v, log_decay, init, lengths = ctx.saved_tensors
+        grads = _ops.linear_attention_bwd(q, k, v, log_decay, init, lengths, ctx.scale, grad_o, grad_state, *need)
+        return (*(g if n else None for g, n in zip(grads, need)), None, None, None)
+
+
+def _normalised(o: Tensor, eps: Optional[float], weight: Optional[Tensor], bias: Optional[Tensor]) -> Tensor:
+    if eps is None:
+        if weight is not None or bias is not None:
+            raise ValueError("norm_weight and norm_bias need norm_eps")
+        return o
+    H, Dv = o.shape[-2:]
+    return layer_norm(o.flatten(-2), weight, bias, eps=eps, groups=H).unflatten(-1, (H, Dv))
+
+
+def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tensor], scale: float,
+           lengths: Optional[Tensor], return_state: Optional[bool], norm_eps: Optional[float],
+           norm_weight: Optional[Tensor], norm_bias: Optional[Tensor]):
+    want = (zi is not None) if return_state is None else bool(return_state)
+    _lib.require_cuda(q, k, v, log_decay, zi, lengths)
+    tensors = (q, k, v, log_decay, zi)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        o, state = LinearAttention.apply(q, k, v, log_decay, zi, lengths, float(scale), want)
+    else:
+        o, state = _ops.linear_attention(q, k, v, log_decay, zi, lengths, float(scale), want)
+    o = _normalised(o, norm_eps, norm_weight, norm_bias)
+    return (o, state) if want else o
+
+
+def attend_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, scale: float,
+                norm_eps: Optional[float], norm_weight: Optional[Tensor], norm_bias: Optional[Tensor]) -> Tensor:
+    _lib.require_cuda(q, k, v, log_decay, state)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise RuntimeError("linear_attention_step updates its state in place and is not differentiable: call it under "
+                           "torch.no_grad(), or linear_attention for gradients")
+    o = _ops.linear_attention_step(q, k, v, log_decay, state, float(scale))
+    return _normalised(o, norm_eps, norm_weight, norm_bias)

@@ -1,0 +1,284 @@
+// C ABI of linear attention with decays (see include/philtorch_b200.h).
+#include "linear_attention.cuh"
+
+namespace ptb {
+
+template <class S> struct LaGeom;
+template <> struct LaGeom<float> { static constexpr int C = 32, NS = 64, PER_SM = 2; };
+template <> struct LaGeom<double> { static constexpr int C = 32, NS = 32, PER_SM = 1; };
+
+constexpr int kLaSms = 148;   // CTAs to aim for; only the cut of the time axis depends on it, never a result's meaning
+
+struct LaPlan {
+  int C, slices_max, nseg, seg_chunks;
+  int64_t nchunk, seg_off, log_off, qb_off, rb_off, qd_off, kd_off, part_off, total;
+  int64_t seg_stride;
+};
+
+// Few (batch, head) pairs: the time axis is cut into segments that run side by side.  Their entering states
+// come from a first pass that only forms the states (it reads two of the three operands), so a cut pays
+// where it at least halves the rows each CTA walks; a segment keeps at least 8 chunks.
+static void la_cut(int64_t ctas, int64_t nchunk, int64_t room, int* nseg, int* seg_chunks) {
+  int64_t n = ctas > 0 ? room / ctas : 1;
+  n = std::min(n, nchunk / 8);
+  if (n < 3) n = 1;
+  int64_t per = n > 1 ? (nchunk + n - 1) / n : std::max<int64_t>(nchunk, 1);
+  *seg_chunks = (int)per;
+  *nseg = n > 1 ? (int)((nchunk + per - 1) / per) : 1;
+}
+
+template <class S>
+static LaPlan la_plan(int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, int roles, bool decay_grad) {
+  using G = LaGeom<S>;
+  LaPlan l;
+  l.C = G::C;
+  l.nchunk = (T + G::C - 1) / G::C;
+  l.slices_max = (kLaMaxDim + G::NS - 1) / G::NS;
+  const int64_t BH = B * H, dmax = std::max(Dk, Dv);
+  la_cut(BH * roles * ((dmax + G::NS - 1) / G::NS), l.nchunk, kLaSms * G::PER_SM, &l.nseg, &l.seg_chunks);
+  l.seg_stride = align_up(Dk * Dv, 64);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t o = at; at = align_up(at + bytes, 256); return o; };
+  l.seg_off = take(l.nseg > 1 ? (int64_t)roles * l.nseg * BH * l.seg_stride * sizeof(S) : 0);
+  l.log_off = take(l.nseg > 1 ? (int64_t)roles * l.nseg * BH * sizeof(double) : 0);
+  l.qb_off = take(decay_grad ? BH * l.nchunk * Dk * Dv * sizeof(S) : 0);
+  l.rb_off = take(decay_grad ? BH * l.nchunk * Dk * Dv * sizeof(S) : 0);
+  l.qd_off = take(decay_grad ? l.slices_max * BH * T * 2 * sizeof(S) : 0);
+  l.kd_off = take(decay_grad ? l.slices_max * BH * T * 2 * sizeof(S) : 0);
+  l.part_off = take(decay_grad ? BH * l.nchunk * sizeof(double) : 0);
+  l.total = std::max<int64_t>(at, 256);
+  return l;
+}
+
+template <class T, class S, bool STATES_ONLY>
+static int la_simt_launch(const LaArgs<S>& a, int roles, cudaStream_t st) {
+  using G = LaGeom<S>;
+  constexpr int smem = sizeof(LaSimtSmem<S, G::C, G::NS>);
+  static bool ready[kMaxDevices] = {};
+  int dev = 0;
+  PTB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return PTB_ERR_ARG;
+  {
+    std::lock_guard<std::mutex> lock(init_mutex());
+    if (!ready[dev]) {
+      PTB_CUDA(cudaFuncSetAttribute(la_simt_kernel<T, S, G::C, G::NS, STATES_ONLY>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      ready[dev] = true;
+    }
+  }
+  const int64_t grid = a.B * a.H * (STATES_ONLY ? a.nseg - 1 : a.nseg) * ((kLaMaxDim + G::NS - 1) / G::NS);
+  if (grid > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
+  la_simt_kernel<T, S, G::C, G::NS, STATES_ONLY><<<dim3((unsigned)grid, roles), 256, smem, st>>>(a);
+  PTB_CUDA(cudaGetLastError());
+  return PTB_OK;
+}
+
+template <class T, class S>
+static int la_run(LaArgs<S>& a, int roles, const LaPlan& l, void* ws, cudaStream_t st) {
+  char* w = static_cast<char*>(ws);
+  a.nseg = l.nseg;
+  a.seg_chunks = l.seg_chunks;
+  a.seg_stride = l.seg_stride;
+  a.seg = reinterpret_cast<S*>(w + l.seg_off);
+  a.seg_log = reinterpret_cast<double*>(w + l.log_off);
+  if (l.nseg > 1) {
+    if (int rc = la_simt_launch<T, S, true>(a, roles, st)) return rc;
+    const int64_t elems = a.B * a.H * (int64_t)a.p[0].M * a.p[0].N;
+    la_join_kernel<S><<<dim3((unsigned)((elems + 255) / 256), roles), 256, 0, st>>>(a);
+    PTB_CUDA(cudaGetLastError());
+  }
+  return la_simt_launch<T, S, false>(a, roles, st);
+}
+
+static void la_strides(int64_t (&d)[3], const int64_t* s) { for (int i = 0; i < 3; ++i) d[i] = s[i]; }
+
+template <class T, class S>
+static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs,
+                  const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
+                  const int64_t* gs, const int32_t* lengths, const void* init, double scale, void* o, void* fin,
+                  void* ws, int64_t wsb, cudaStream_t st) {
+  const LaPlan l = la_plan<S>(B, T_, H, Dk, Dv, 1, false);
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total) return PTB_ERR_WORKSPACE;
+  LaArgs<S> a = {};
+  LaPass<S>& p = a.p[0];
+  p.x = q; p.y = k; p.z = v;
+  la_strides(p.xs, qs); la_strides(p.ys, ks); la_strides(p.zs, vs);
+  p.o = o;
+  p.init = static_cast<const S*>(init);
+  p.fin = static_cast<S*>(fin);
+  p.M = (int)Dk; p.N = (int)Dv;
+  p.po = (S)scale; p.pz = (S)1;
+  a.g = static_cast<const S*>(g);
+  la_strides(a.gs, gs);
+  a.lengths = lengths;
+  a.B = B; a.T = T_; a.H = H;
+  return la_run<T, S>(a, 1, l, ws, st);
+}
+
+template <class T, class S>
+static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs,
+                  const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
+                  const int64_t* gs, const int32_t* lengths, const void* init, double scale, const void* go,
+                  const int64_t* gos, const void* gfin, void* gq, void* gk, void* gv, void* gg, int gg_per_token,
+                  void* ginit, void* ws, int64_t wsb, cudaStream_t st) {
+  const bool dec = gg != nullptr;
+  const LaPlan l = la_plan<S>(B, T_, H, Dk, Dv, 3, dec);
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total) return PTB_ERR_WORKSPACE;
+  char* w = static_cast<char*>(ws);
+  LaArgs<S> a = {};
+  a.g = static_cast<const S*>(g);
+  la_strides(a.gs, gs);
+  a.lengths = lengths;
+  a.B = B; a.T = T_; a.H = H;
+  int roles = 0;
+  if (gq || dec) {
+    LaPass<S>& p = a.p[roles++];
+    p.x = go; p.y = v; p.z = k; p.w = q;
+    la_strides(p.xs, gos); la_strides(p.ys, vs); la_strides(p.zs, ks); la_strides(p.ws, qs);
+    p.o = gq;
+    p.init = static_cast<const S*>(init);
+    p.M = (int)Dv; p.N = (int)Dk; p.state_t = 1;
+    p.po = (S)scale; p.pz = (S)1;
+    if (dec) { p.bounds = reinterpret_cast<S*>(w + l.qb_off); p.dots = reinterpret_cast<S*>(w + l.qd_off); }
+  }
+  if (gk || dec || ginit) {
+    LaPass<S>& p = a.p[roles++];
+    p.x = v; p.y = go; p.z = q; p.w = k;
+    la_strides(p.xs, vs); la_strides(p.ys, gos); la_strides(p.zs, qs); la_strides(p.ws, ks);
+    p.o = gk;
+    p.init = static_cast<const S*>(gfin);
+    p.fin = static_cast<S*>(ginit);
+    p.M = (int)Dv; p.N = (int)Dk; p.state_t = 1; p.reverse = 1;
+    p.po = (S)1; p.pz = (S)scale;
+    if (dec) { p.bounds = reinterpret_cast<S*>(w + l.rb_off); p.dots = reinterpret_cast<S*>(w + l.kd_off); }
+  }
+  if (gv) {
+    LaPass<S>& p = a.p[roles++];
+    p.x = k; p.y = q; p.z = go;
+    la_strides(p.xs, ks); la_strides(p.ys, qs); la_strides(p.zs, gos);
+    p.o = gv;
+    p.init = static_cast<const S*>(gfin);
+    p.M = (int)Dk; p.N = (int)Dv; p.reverse = 1;
+    p.po = (S)1; p.pz = (S)scale;
+  }
+  if (roles == 0) return PTB_OK;
+  if (int rc = la_run<T, S>(a, roles, l, ws, st)) return rc;
+  if (dec && l.nchunk > 0) {
+    LaDecayArgs<S> d = {};
+    d.s_bounds = reinterpret_cast<const S*>(w + l.qb_off);
+    d.r_bounds = reinterpret_cast<const S*>(w + l.rb_off);
+    d.qd = reinterpret_cast<const S*>(w + l.qd_off);
+    d.kd = reinterpret_cast<const S*>(w + l.kd_off);
+    d.q_slices = d.k_slices = (int)((Dk + LaGeom<S>::NS - 1) / LaGeom<S>::NS);
+    d.g = a.g;
+    la_strides(d.gs, gs);
+    d.lengths = lengths;
+    d.B = B; d.T = T_; d.H = H; d.MN = Dk * Dv;
+    if (gg_per_token) d.dg = static_cast<S*>(gg);
+    else d.part = reinterpret_cast<double*>(w + l.part_off);
+    if (B * H * l.nchunk > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
+    la_decay_grad_kernel<S, LaGeom<S>::C><<<(unsigned)(B * H * l.nchunk), 256, 0, st>>>(d);
+    PTB_CUDA(cudaGetLastError());
+  }
+  if (dec && !gg_per_token) {
+    la_decay_sum_kernel<S><<<(unsigned)H, 256, 0, st>>>(reinterpret_cast<double*>(w + l.part_off), l.nchunk, B, H,
+                                                         static_cast<S*>(gg));
+    PTB_CUDA(cudaGetLastError());
+  }
+  return PTB_OK;
+}
+
+template <class T, class S>
+static int la_step(int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs, const void* k,
+                   const int64_t* ks, const void* v, const int64_t* vs, const void* g, const int64_t* gs, double scale,
+                   void* state, const int64_t* ss, void* o, cudaStream_t st) {
+  LaStepArgs<T, S> a;
+  a.q = static_cast<const T*>(q); a.k = static_cast<const T*>(k); a.v = static_cast<const T*>(v);
+  for (int i = 0; i < 2; ++i) { a.qs[i] = qs[i]; a.ks[i] = ks[i]; a.vs[i] = vs[i]; a.gs[i] = gs[i]; a.ss[i] = ss[i]; }
+  a.g = static_cast<const S*>(g);
+  a.state = static_cast<S*>(state);
+  a.o = static_cast<T*>(o);
+  a.H = H; a.M = (int)Dk; a.N = (int)Dv;
+  a.scale = (S)scale;
+  constexpr int V = 16 / sizeof(S);
+  const dim3 grid((unsigned)(B * H), (unsigned)((Dv + 31) / 32));
+  if (aligned16(state) && Dv % V == 0 && ss[0] % V == 0 && ss[1] % V == 0) la_step_kernel<T, S, V><<<grid, 256, 0, st>>>(a);
+  else la_step_kernel<T, S, 1><<<grid, 256, 0, st>>>(a);
+  PTB_CUDA(cudaGetLastError());
+  return PTB_OK;
+}
+
+static int la_check(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv) {
+  if (dtype != PTB_F32 && dtype != PTB_F64 && dtype != PTB_F16 && dtype != PTB_BF16) return PTB_ERR_ARG;
+  if (B < 0 || T < 0 || H < 0 || Dk < 1 || Dv < 1 || Dk > kLaMaxDim || Dv > kLaMaxDim) return PTB_ERR_ARG;
+  if (B > 0x7fffffffll || H > 0x7fffffffll || B * H > 0x7fffffffll || T > (1ll << 40)) return PTB_ERR_TOO_LARGE;
+  return PTB_OK;
+}
+
+}  // namespace ptb
+
+using namespace ptb;
+
+#define PTB_LA_TYPES(CALL)                                                                   \
+  switch (dtype) {                                                                           \
+    case PTB_F64: { using T_ = double; using S_ = double; return CALL; }                     \
+    case PTB_F32: { using T_ = float; using S_ = float; return CALL; }                       \
+    case PTB_F16: { using T_ = __half; using S_ = float; return CALL; }                      \
+    default: { using T_ = __nv_bfloat16; using S_ = float; return CALL; }                    \
+  }
+
+extern "C" {
+
+int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
+                                             int backward, int decay_grad) {
+  if (la_check(dtype, B, T, H, Dk, Dv) != PTB_OK) return 0;
+  const int roles = backward ? 3 : 1;
+  return dtype == PTB_F64 ? la_plan<double>(B, T, H, Dk, Dv, roles, decay_grad).total
+                          : la_plan<float>(B, T, H, Dk, Dv, roles, decay_grad).total;
+}
+
+int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                             const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                             const int32_t* lengths, const void* init, double scale, void* o, void* fin,
+                             void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
+  (void)status;
+  if (int rc = la_check(dtype, B, T, H, Dk, Dv)) return rc;
+  if (B == 0 || H == 0) return PTB_OK;
+  if ((T > 0 && (!q || !k || !v || !o || !log_decay)) || !q_strides || !k_strides || !v_strides || !log_decay_strides) return PTB_ERR_ARG;
+  PTB_LA_TYPES((la_fwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
+                               lengths, init, scale, o, fin, workspace, workspace_bytes, (cudaStream_t)stream)))
+}
+
+int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                             const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                             const int32_t* lengths, const void* init, double scale, const void* grad_o,
+                             const int64_t* grad_o_strides, const void* grad_fin, void* grad_q, void* grad_k,
+                             void* grad_v, void* grad_log_decay, int grad_log_decay_per_token, void* grad_init,
+                             void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
+  (void)status;
+  if (int rc = la_check(dtype, B, T, H, Dk, Dv)) return rc;
+  if (B == 0 || H == 0) return PTB_OK;
+  if ((T > 0 && (!q || !k || !v || !log_decay || !grad_o)) || !q_strides || !k_strides || !v_strides || !log_decay_strides ||
+      !grad_o_strides)
+    return PTB_ERR_ARG;
+  PTB_LA_TYPES((la_bwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
+                               lengths, init, scale, grad_o, grad_o_strides, grad_fin, grad_q, grad_k, grad_v,
+                               grad_log_decay, grad_log_decay_per_token, grad_init, workspace, workspace_bytes,
+                               (cudaStream_t)stream)))
+}
+
+int ptb_linear_attention_step(int dtype, int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                              double scale, void* state, const int64_t* state_strides, void* o, ptb_stream_t stream) {
+  if (int rc = la_check(dtype, B, 1, H, Dk, Dv)) return rc;
+  if (B == 0 || H == 0) return PTB_OK;
+  if (!q || !k || !v || !log_decay || !state || !o || !q_strides || !k_strides || !v_strides || !log_decay_strides || !state_strides)
+    return PTB_ERR_ARG;
+  PTB_LA_TYPES((la_step<T_, S_>(B, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
+                                scale, state, state_strides, o, (cudaStream_t)stream)))
+}
+
+}  // extern "C"

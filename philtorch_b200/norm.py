@@ -1,0 +1,155 @@
+"""Layer norm over groups of channels: the read-out normalisation of ``linear_attention`` (one group per
+head), and the norm over whole rows (one group)."""
+from __future__ import annotations
+
+from typing import Any, Optional
+
+import torch
+from torch import Tensor
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import lib, ptr
+from .ops import _LIB, _TAGS
+
+__all__ = ["LayerNorm", "layer_norm", "MAX_WIDTH"]
+
+MAX_WIDTH = 16384
+_CODES = {torch.float32: _lib.PTB_F32, torch.float64: _lib.PTB_F64, torch.float16: _lib.PTB_F16,
+          torch.bfloat16: _lib.PTB_BF16}
+
+_LIB.define("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, int groups) -> (Tensor, Tensor, Tensor)",
+            tags=_TAGS)
+_LIB.define("layer_norm_bwd(Tensor x, Tensor? weight, Tensor? bias, Tensor mean, Tensor rstd, Tensor grad_y, int groups, "
+            "bool need_x, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)", tags=_TAGS)
+
+
+def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int) -> None:
+    torch._check(x.dim() >= 1, lambda: "x must have at least one axis")
+    C = x.shape[-1]
+    torch._check(1 <= groups <= 65535 and C % groups == 0 and C > 0,
+                 lambda: f"the last axis ({C}) must be a multiple of groups ({groups}, at most 65535)")
+    torch._check(C // groups <= MAX_WIDTH, lambda: f"groups of {C // groups} channels: the kernels cover 1..{MAX_WIDTH}.")
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            torch._check(tuple(p.shape) == (C,), lambda: f"{name} must be ({C},), got {tuple(p.shape)}")
+            torch._check(p.dtype in (x.dtype, wide), lambda: f"{name} must be {x.dtype} or {wide}, got {p.dtype}")
+    if weight is not None and bias is not None:
+        torch._check(weight.dtype == bias.dtype,
+                     lambda: f"weight and bias must have the same type, got {weight.dtype} and {bias.dtype}")
+
+
+def _code(t: Tensor) -> int:
+    try:
+        return _CODES[t.dtype]
+    except KeyError:
+        raise RuntimeError(f"layer_norm takes float32, float64, float16 and bfloat16 tensors, got {t.dtype}") from None
+
+
+def _as_rows(t: Tensor) -> Tensor:
+    """(rows, channels) with dense channels; a view where the strides allow it."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _wide(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> int:
+    p = weight if weight is not None else bias
+    return int(p is not None and p.dtype in (torch.float32, torch.float64))
+
+
+def _layer_norm(x, weight, bias, eps, groups):
+    _check(x, weight, bias, groups)
+    dev = _lib.require_cuda(x, weight, bias)
+    rows = _as_rows(x)
+    R, C = rows.shape
+    w, b = (None if p is None else p.contiguous() for p in (weight, bias))
+    y = x.new_empty(x.shape)
+    stats = torch.empty((2, R, groups), dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=x.device)
+    if R:
+        _lib.launch(lib.ptb_layer_norm_fwd, dev, _code(x), R, groups, C // groups, ptr(rows), rows.stride(0), ptr(w), ptr(b),
+                    _wide(x, weight, bias), eps, ptr(y), ptr(stats), stats.data_ptr() + stats.stride(0) * stats.element_size())
+    return y, stats[0], stats[1]
+
+
+def _layer_norm_bwd(x, weight, bias, mean, rstd, grad_y, groups, need_x, need_weight, need_bias):
+    dev = _lib.require_cuda(x, weight, bias, mean, rstd, grad_y)
+    rows, gy = _as_rows(x), _as_rows(grad_y)
+    R, C = rows.shape
+    w = None if weight is None else weight.contiguous()
+    gx = x.new_empty(x.shape if need_x else (0,))
+    gw = weight.new_empty((C,)) if need_weight else x.new_empty(0)
+    gb = bias.new_empty((C,)) if need_bias else x.new_empty(0)
+    if R:
+        code, width = _code(x), C // groups
+        ws = lib.ptb_layer_norm_bwd_workspace_bytes(code, R, groups, width) if need_weight or need_bias else 0
+        _lib.call(lib.ptb_layer_norm_bwd, dev, R, C, code, R, groups, width, ptr(rows), rows.stride(0), ptr(w),
+                  _wide(x, weight, bias), ptr(mean.contiguous()), ptr(rstd.contiguous()), ptr(gy), gy.stride(0),
+                  ptr(gx) if need_x else None, ptr(gw) if need_weight else None, ptr(gb) if need_bias else None, ws_bytes=ws)
+    else:
+        gw.zero_()
+        gb.zero_()
+    return gx, gw, gb
+
+
+_LIB.impl("layer_norm", _layer_norm, "CUDA")
+_LIB.impl("layer_norm_bwd", _layer_norm_bwd, "CUDA")
+
+
+@torch.library.register_fake("philtorch_b200::layer_norm")
+def _(x, weight, bias, eps, groups):
+    _check(x, weight, bias, groups)
+    rows = x.numel() // x.shape[-1]
+    stats = torch.float64 if x.dtype == torch.float64 else torch.float32
+    return x.new_empty(x.shape), x.new_empty((rows, groups), dtype=stats), x.new_empty((rows, groups), dtype=stats)
+
+
+@torch.library.register_fake("philtorch_b200::layer_norm_bwd")
+def _(x, weight, bias, mean, rstd, grad_y, groups, need_x, need_weight, need_bias):
+    C = x.shape[-1]
+    return (x.new_empty(x.shape if need_x else (0,)), weight.new_empty((C,)) if need_weight else x.new_empty(0),
+            bias.new_empty((C,)) if need_bias else x.new_empty(0))
+
+
+_ops = torch.ops.philtorch_b200
+
+
+class LayerNorm(Function):
+    """(x, weight or None, bias or None, eps, groups) -> y; first derivatives."""
+
+    @staticmethod
+    def forward(ctx: Any, x, weight, bias, eps: float, groups: int):
+        y, mean, rstd = _ops.layer_norm(x, weight, bias, eps, groups)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.groups = groups
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad_y: Tensor):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad[:3]
+        grads = _ops.layer_norm_bwd(x, weight, bias, mean, rstd, grad_y, ctx.groups, *need)
+        return (*(g if n else None for g, n in zip(grads, need)), None, None)
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
+               groups: int = 1) -> Tensor:
+    """Normalises groups of consecutive channels of the last axis to mean zero and variance one, then applies
+    a weight and a bias per channel.
+
+    Args:
+        x: (..., C), CUDA, float32, float64, float16 or bfloat16 (statistics in float32 or better).
+        weight, bias: (C,) of x's type or float32 (float64 beside float64), or None.
+        eps: added to the variance.
+        groups: the last axis is cut into this many groups of C / groups <= 16384 channels; 1: whole rows.
+
+    Returns:
+        Tensor of x's shape and type.  Differentiable once in x, weight and bias; their gradients are sums
+        in a fixed order (bit-reproducible).
+    """
+    _lib.require_cuda(x, weight, bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return LayerNorm.apply(x, weight, bias, float(eps), int(groups))
+    return _ops.layer_norm(x, weight, bias, float(eps), int(groups))[0]
