@@ -1,5 +1,6 @@
 // C ABI of linear attention with decays (see include/philtorch_b200.h).
 #include "linear_attention.cuh"
+#include "linear_attention_mma.cuh"
 
 namespace ptb {
 
@@ -12,7 +13,7 @@ constexpr int kLaSms = 148;   // CTAs to aim for; only the cut of the time axis 
 struct LaPlan {
   int C, slices_max, nseg, seg_chunks;
   int64_t nchunk, seg_off, log_off, qb_off, rb_off, qd_off, kd_off, part_off, total;
-  int64_t seg_stride;
+  int64_t seg_stride, bound_elems;
 };
 
 // Few (batch, head) pairs: the time axis is cut into segments that run side by side.  Their entering states
@@ -27,27 +28,48 @@ static void la_cut(int64_t ctas, int64_t nchunk, int64_t room, int* nseg, int* s
   *nseg = n > 1 ? (int)((nchunk + per - 1) / per) : 1;
 }
 
+struct LaSize { int64_t B, T, H, Dk, Dv; };
+
+// C: tokens of a chunk; slices: CTAs that share the columns of a state; mn: scalars of a stored state
 template <class S>
-static LaPlan la_plan(int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, int roles, bool decay_grad) {
-  using G = LaGeom<S>;
+static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int slices, int64_t mn, int per_sm, int slots) {
   LaPlan l;
-  l.C = G::C;
-  l.nchunk = (T + G::C - 1) / G::C;
-  l.slices_max = (kLaMaxDim + G::NS - 1) / G::NS;
-  const int64_t BH = B * H, dmax = std::max(Dk, Dv);
-  la_cut(BH * roles * ((dmax + G::NS - 1) / G::NS), l.nchunk, kLaSms * G::PER_SM, &l.nseg, &l.seg_chunks);
-  l.seg_stride = align_up(Dk * Dv, 64);
+  l.C = C;
+  l.slices_max = slices;
+  l.nchunk = (z.T + C - 1) / C;
+  const int64_t BH = z.B * z.H;
+  la_cut(BH * roles * slices, l.nchunk, kLaSms * per_sm, &l.nseg, &l.seg_chunks);
+  l.seg_stride = align_up(mn, 64);
+  l.bound_elems = mn;
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at = align_up(at + bytes, 256); return o; };
-  l.seg_off = take(l.nseg > 1 ? (int64_t)roles * l.nseg * BH * l.seg_stride * sizeof(S) : 0);
+  l.seg_off = take(l.nseg > 1 ? (int64_t)roles * (l.nseg + slots) * BH * l.seg_stride * sizeof(S) : 0);
   l.log_off = take(l.nseg > 1 ? (int64_t)roles * l.nseg * BH * sizeof(double) : 0);
-  l.qb_off = take(decay_grad ? BH * l.nchunk * Dk * Dv * sizeof(S) : 0);
-  l.rb_off = take(decay_grad ? BH * l.nchunk * Dk * Dv * sizeof(S) : 0);
-  l.qd_off = take(decay_grad ? l.slices_max * BH * T * 2 * sizeof(S) : 0);
-  l.kd_off = take(decay_grad ? l.slices_max * BH * T * 2 * sizeof(S) : 0);
+  l.qb_off = take(decay_grad ? BH * l.nchunk * mn * sizeof(S) : 0);
+  l.rb_off = take(decay_grad ? BH * l.nchunk * mn * sizeof(S) : 0);
+  l.qd_off = take(decay_grad ? l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
+  l.kd_off = take(decay_grad ? l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
   l.part_off = take(decay_grad ? BH * l.nchunk * sizeof(double) : 0);
   l.total = std::max<int64_t>(at, 256);
   return l;
+}
+template <class S>
+static LaPlan la_simt_plan(const LaSize& z, int roles, bool decay_grad) {
+  using G = LaGeom<S>;
+  return la_plan<S>(z, roles, decay_grad, G::C, (int)((std::max(z.Dk, z.Dv) + G::NS - 1) / G::NS), z.Dk * z.Dv, G::PER_SM, 0);
+}
+// the tensor-core kernels come for head sizes up to 64 and up to 128
+static int la_mma_width(const LaSize& z) { return std::max(z.Dk, z.Dv) <= 64 ? 64 : 128; }
+static LaPlan la_mma_plan(const LaSize& z, int roles, bool decay_grad) {
+  const int64_t W = la_mma_width(z);
+  return la_plan<float>(z, roles, decay_grad, kLaMmaChunk, 1, W * W, W == 64 ? 4 : 2, 1);
+}
+// which kernels a type runs on
+template <class T> constexpr bool kLaMma = std::is_same<T, __nv_bfloat16>::value;
+template <class T, class S>
+static LaPlan la_plan_of(const LaSize& z, int roles, bool decay_grad) {
+  if constexpr (kLaMma<T>) return la_mma_plan(z, roles, decay_grad);
+  else return la_simt_plan<S>(z, roles, decay_grad);
 }
 
 template <class T, class S, bool STATES_ONLY>
@@ -73,21 +95,97 @@ static int la_simt_launch(const LaArgs<S>& a, int roles, cudaStream_t st) {
   return PTB_OK;
 }
 
-template <class T, class S>
-static int la_run(LaArgs<S>& a, int roles, const LaPlan& l, void* ws, cudaStream_t st) {
+template <class S>
+static void la_workspace(LaArgs<S>& a, const LaPlan& l, void* ws) {
   char* w = static_cast<char*>(ws);
   a.nseg = l.nseg;
   a.seg_chunks = l.seg_chunks;
   a.seg_stride = l.seg_stride;
   a.seg = reinterpret_cast<S*>(w + l.seg_off);
   a.seg_log = reinterpret_cast<double*>(w + l.log_off);
-  if (l.nseg > 1) {
+}
+
+template <class T, class S>
+static int la_simt_run(LaArgs<S>& a, int roles, cudaStream_t st) {
+  if (a.nseg > 1) {
     if (int rc = la_simt_launch<T, S, true>(a, roles, st)) return rc;
     const int64_t elems = a.B * a.H * (int64_t)a.p[0].M * a.p[0].N;
     la_join_kernel<S><<<dim3((unsigned)((elems + 255) / 256), roles), 256, 0, st>>>(a);
     PTB_CUDA(cudaGetLastError());
   }
   return la_simt_launch<T, S, false>(a, roles, st);
+}
+
+template <int W, bool VEC, bool STATES_ONLY>
+static int la_mma_launch(const LaArgs<float>& a, const LaMmaFlags& f, int roles, bool dots, cudaStream_t st) {
+  static bool ready[kMaxDevices] = {};
+  int dev = 0;
+  PTB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return PTB_ERR_ARG;
+  const int smem = LaMmaSmem<W, W>::bytes(f.stages, dots);
+  {
+    std::lock_guard<std::mutex> lock(init_mutex());
+    if (!ready[dev]) {
+      PTB_CUDA(cudaFuncSetAttribute(la_mma_kernel<W, W, VEC, STATES_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    LaMmaSmem<W, W>::bytes(2, false)));   // the most that is ever asked for
+      ready[dev] = true;
+    }
+  }
+  const int64_t grid = a.B * a.H * (STATES_ONLY ? a.nseg - (f.all_segments ? 0 : 1) : a.nseg);
+  if (grid > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
+  la_mma_kernel<W, W, VEC, STATES_ONLY><<<dim3((unsigned)grid, roles), 128, smem, st>>>(a, f);
+  PTB_CUDA(cudaGetLastError());
+  return PTB_OK;
+}
+
+template <int W, bool VEC>
+static int la_mma_run(const LaArgs<float>& a, int roles, bool dots, cudaStream_t st) {
+  LaMmaFlags main = {}, states = {};
+  // one buffer of the operands beside w, else two: either way two CTAs fit an SM
+  main.stages = dots ? 1 : 2;
+  states.stages = 2;
+  for (int r = 0; r < roles; ++r) {
+    // with dots, the states kept at the chunks' ends and what is read from them are float32 results; otherwise
+    // only the final state is one, and where the row is cut, the pass that forms the segments' states gives it
+    const bool exact = a.p[r].dots, end = a.p[r].fin && !exact;
+    main.accurate[r] = exact ? 3 : end && a.nseg == 1 ? 1 : 0;
+    states.accurate[r] = exact || end ? 1 : 0;
+    if (end && a.nseg > 1) main.all_segments = states.all_segments = 1;
+  }
+  if (a.nseg > 1) {
+    if (int rc = la_mma_launch<W, VEC, true>(a, states, roles, false, st)) return rc;
+    const int64_t elems = a.B * a.H * W * W;
+    if (elems / 256 > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
+    la_mma_join_kernel<W, W><<<dim3((unsigned)((elems + 255) / 256), roles), 256, 0, st>>>(a, states);
+    PTB_CUDA(cudaGetLastError());
+  }
+  return la_mma_launch<W, VEC, false>(a, main, roles, dots, st);
+}
+
+// 16-byte accesses: every operand's rows start on 16 bytes and hold a multiple of 8 values
+static bool la_mma_vec(const LaArgs<float>& a, int roles) {
+  for (int r = 0; r < roles; ++r) {
+    const LaPass<float>& p = a.p[r];
+    if (p.M % 8 || p.N % 8 || !aligned16(p.x) || !aligned16(p.y) || !aligned16(p.z) || !aligned16(p.w) || !aligned16(p.o)) return false;
+    for (int i = 0; i < 3; ++i)
+      if (p.xs[i] % 8 || p.ys[i] % 8 || p.zs[i] % 8 || p.ws[i] % 8) return false;
+  }
+  return true;
+}
+
+template <class T, class S>
+static int la_run(LaArgs<S>& a, int roles, const LaPlan& l, void* ws, cudaStream_t st) {
+  la_workspace(a, l, ws);
+  if constexpr (kLaMma<T>) {
+    bool dots = false;
+    for (int r = 0; r < roles; ++r) dots = dots || a.p[r].dots;
+    const bool vec = la_mma_vec(a, roles);
+    if (std::max(a.p[0].M, a.p[0].N) <= 64)
+      return vec ? la_mma_run<64, true>(a, roles, dots, st) : la_mma_run<64, false>(a, roles, dots, st);
+    return vec ? la_mma_run<128, true>(a, roles, dots, st) : la_mma_run<128, false>(a, roles, dots, st);
+  } else {
+    return la_simt_run<T, S>(a, roles, st);
+  }
 }
 
 static void la_strides(int64_t (&d)[3], const int64_t* s) { for (int i = 0; i < 3; ++i) d[i] = s[i]; }
@@ -97,7 +195,7 @@ static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
                   const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
                   const int64_t* gs, const int32_t* lengths, const void* init, double scale, void* o, void* fin,
                   void* ws, int64_t wsb, cudaStream_t st) {
-  const LaPlan l = la_plan<S>(B, T_, H, Dk, Dv, 1, false);
+  const LaPlan l = la_plan_of<T, S>({B, T_, H, Dk, Dv}, 1, false);
   if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total) return PTB_ERR_WORKSPACE;
   LaArgs<S> a = {};
   LaPass<S>& p = a.p[0];
@@ -122,7 +220,7 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
                   const int64_t* gos, const void* gfin, void* gq, void* gk, void* gv, void* gg, int gg_per_token,
                   void* ginit, void* ws, int64_t wsb, cudaStream_t st) {
   const bool dec = gg != nullptr;
-  const LaPlan l = la_plan<S>(B, T_, H, Dk, Dv, 3, dec);
+  const LaPlan l = la_plan_of<T, S>({B, T_, H, Dk, Dv}, 3, dec);
   if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total) return PTB_ERR_WORKSPACE;
   char* w = static_cast<char*>(ws);
   LaArgs<S> a = {};
@@ -169,15 +267,15 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
     d.r_bounds = reinterpret_cast<const S*>(w + l.rb_off);
     d.qd = reinterpret_cast<const S*>(w + l.qd_off);
     d.kd = reinterpret_cast<const S*>(w + l.kd_off);
-    d.q_slices = d.k_slices = (int)((Dk + LaGeom<S>::NS - 1) / LaGeom<S>::NS);
+    d.q_slices = d.k_slices = kLaMma<T> ? 1 : (int)((Dk + LaGeom<S>::NS - 1) / LaGeom<S>::NS);
     d.g = a.g;
     la_strides(d.gs, gs);
     d.lengths = lengths;
-    d.B = B; d.T = T_; d.H = H; d.MN = Dk * Dv;
+    d.B = B; d.T = T_; d.H = H; d.MN = l.bound_elems;
     if (gg_per_token) d.dg = static_cast<S*>(gg);
     else d.part = reinterpret_cast<double*>(w + l.part_off);
     if (B * H * l.nchunk > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
-    la_decay_grad_kernel<S, LaGeom<S>::C><<<(unsigned)(B * H * l.nchunk), 256, 0, st>>>(d);
+    la_decay_grad_kernel<S, kLaMma<T> ? kLaMmaChunk : LaGeom<S>::C><<<(unsigned)(B * H * l.nchunk), 256, 0, st>>>(d);
     PTB_CUDA(cudaGetLastError());
   }
   if (dec && !gg_per_token) {
@@ -232,9 +330,9 @@ extern "C" {
 int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
                                              int backward, int decay_grad) {
   if (la_check(dtype, B, T, H, Dk, Dv) != PTB_OK) return 0;
+  const LaSize z = {B, T, H, Dk, Dv};
   const int roles = backward ? 3 : 1;
-  return dtype == PTB_F64 ? la_plan<double>(B, T, H, Dk, Dv, roles, decay_grad).total
-                          : la_plan<float>(B, T, H, Dk, Dv, roles, decay_grad).total;
+  PTB_LA_TYPES((la_plan_of<T_, S_>(z, roles, decay_grad).total))
 }
 
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
