@@ -3,6 +3,7 @@
 
 #include "comb.cuh"
 #include "comb_slab.cuh"
+#include "tensor_map.cuh"
 
 namespace ptb {
 
@@ -35,24 +36,6 @@ static bool comb_slab_ok(int64_t N, int64_t D, std::initializer_list<const void*
 constexpr int64_t kSmemPerSm = 228 * 1024, kSmemPerCtaMax = 227 * 1024, kSmemCtaOverhead = 1024;
 
 // ---- tensor maps: (phase, step, row) view of a (B, N) signal, box W x KS x 1 ------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn tensor_map_encoder() {
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  std::lock_guard<std::mutex> init_lock(init_mutex());
-  if (!tried) {
-    tried = true;
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(sym);
-  }
-  return fn;
-}
-
 template <class S>
 static bool comb_tensor_map(CUtensorMap* map, const void* base, int64_t B, int64_t N, int64_t D, int64_t K, int W,
                             int KS) {

@@ -1,6 +1,7 @@
 // C ABI of linear attention with decays (see include/philtorch_b200.h).
 #include "linear_attention.cuh"
 #include "linear_attention_mma.cuh"
+#include "linear_attention_tc.cuh"
 
 namespace ptb {
 
@@ -47,8 +48,8 @@ static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int sl
   l.log_off = take(l.nseg > 1 ? (int64_t)roles * l.nseg * BH * sizeof(double) : 0);
   l.qb_off = take(decay_grad ? BH * l.nchunk * mn * sizeof(S) : 0);
   l.rb_off = take(decay_grad ? BH * l.nchunk * mn * sizeof(S) : 0);
-  l.qd_off = take(decay_grad ? l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
-  l.kd_off = take(decay_grad ? l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
+  l.qd_off = take(decay_grad ? 2 * l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
+  l.kd_off = take(decay_grad ? 2 * l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
   l.part_off = take(decay_grad ? BH * l.nchunk * sizeof(double) : 0);
   l.total = std::max<int64_t>(at, 256);
   return l;
@@ -64,12 +65,17 @@ static LaPlan la_mma_plan(const LaSize& z, int roles, bool decay_grad) {
   const int64_t W = la_mma_width(z);
   return la_plan<float>(z, roles, decay_grad, kLaMmaChunk, 1, W * W, W == 64 ? 4 : 2, 1);
 }
-// which kernels a type runs on
-template <class T> constexpr bool kLaMma = std::is_same<T, __nv_bfloat16>::value;
-template <class T, class S>
-static LaPlan la_plan_of(const LaSize& z, int roles, bool decay_grad) {
-  if constexpr (kLaMma<T>) return la_mma_plan(z, roles, decay_grad);
-  else return la_simt_plan<S>(z, roles, decay_grad);
+static LaPlan la_tc_plan(const LaSize& z, int roles, bool decay_grad) {
+  return la_plan<float>(z, roles, decay_grad, kTcChunk, 2, kTcDim * kTcDim, 1, 1);
+}
+enum LaPath { kLaSimt, kLaMma, kLaTc };
+template <class S>
+static LaPlan la_plan_of(LaPath path, const LaSize& z, int roles, bool decay_grad) {
+  if constexpr (std::is_same<S, float>::value) {
+    if (path == kLaMma) return la_mma_plan(z, roles, decay_grad);
+    if (path == kLaTc) return la_tc_plan(z, roles, decay_grad);
+  }
+  return la_simt_plan<S>(z, roles, decay_grad);
 }
 
 template <class T, class S, bool STATES_ONLY>
@@ -173,10 +179,118 @@ static bool la_mma_vec(const LaArgs<float>& a, int roles) {
   return true;
 }
 
+// ---- tcgen05 kernels
+// (Dv | Dk, T, H, B) view of an operand, box 64 x 128 tokens; an axis of stride zero (or of one entry) is left out
+static bool la_tc_map(LaTcMap* m, const void* base, const int64_t* st, int64_t B, int64_t T, int64_t H, int64_t D) {
+  const EncodeTiledFn enc = tensor_map_encoder();
+  if (!enc || !base) return false;
+  m->bmul = B > 1 && st[0] != 0;
+  m->hmul = H > 1 && st[2] != 0;
+  const int64_t ts = T > 1 ? st[1] : D;
+  if (ts == 0 && T > 1) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)(m->hmul ? H : 1), (cuuint64_t)(m->bmul ? B : 1)};
+  const cuuint64_t strides[3] = {(cuuint64_t)(T > 1 ? ts * 2 : 16), (cuuint64_t)(m->hmul ? st[2] * 2 : 16),
+                                 (cuuint64_t)(m->bmul ? st[0] * 2 : 16)};
+  for (cuuint64_t v : strides)
+    if (v % 16 || v >= (1ull << 40)) return false;
+  const cuuint32_t box[4] = {64u, (cuuint32_t)kTcChunk, 1u, 1u}, estr[4] = {1u, 1u, 1u, 1u};
+  return enc(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The tcgen05 kernels take head sizes above 64 (their tiles are 128 wide; up to 64 the mma.sync kernels do half the
+// work) and operands that the TMA unit can address.
+static bool la_tc_setup(LaTcArgs* k, const LaArgs<float>& a, int roles) {
+  if (std::max(a.p[0].M, a.p[0].N) <= 64 || a.T < 1 || a.T > 0x7fffffffll || !la_mma_vec(a, roles)) return false;
+  for (int r = 0; r < roles; ++r) {
+    const LaPass<float>& p = a.p[r];
+    if (!la_tc_map(&k->x[r], p.x, p.xs, a.B, a.T, a.H, p.M) || !la_tc_map(&k->y[r], p.y, p.ys, a.B, a.T, a.H, p.M) ||
+        !la_tc_map(&k->z[r], p.z, p.zs, a.B, a.T, a.H, p.N))
+      return false;
+    if (p.w && !la_tc_map(&k->w[r], p.w, p.ws, a.B, a.T, a.H, p.N)) return false;
+  }
+  return true;
+}
+
+template <bool STATES_ONLY, bool DOTS>
+static int la_tc_launch(const LaTcArgs& k, int roles, cudaStream_t st) {
+  static bool ready[kMaxDevices] = {};
+  int dev = 0;
+  PTB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return PTB_ERR_ARG;
+  const int smem = LaTcSmem(k.xy_stages, DOTS, 3, DOTS ? 3 : 1).total;
+  {
+    std::lock_guard<std::mutex> lock(init_mutex());
+    if (!ready[dev]) {
+      PTB_CUDA(cudaFuncSetAttribute(la_tc_kernel<STATES_ONLY, DOTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      ready[dev] = true;
+    }
+  }
+  const int64_t grid = k.a.B * k.a.H * 2 * (STATES_ONLY ? k.a.nseg - (k.all_segments ? 0 : 1) : k.a.nseg);
+  if (grid > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
+  la_tc_kernel<STATES_ONLY, DOTS><<<dim3((unsigned)grid, roles), kTcThreads, smem, st>>>(k);
+  PTB_CUDA(cudaGetLastError());
+  return PTB_OK;
+}
+
+// roles [0, exact) have dots
+static int la_tc_run(LaTcArgs& k, int roles, cudaStream_t st) {
+  const LaArgs<float>& a = k.a;
+  bool dots = false;
+  for (int r = 0; r < roles; ++r) {
+    const bool exact = a.p[r].dots, end = a.p[r].fin && !exact;
+    dots = dots || exact;
+    k.ns[r] = exact ? 3 : 1;
+    k.nu[r] = exact || end ? 3 : 2;
+    if (end && a.nseg > 1) k.all_segments = 1;
+  }
+  if (a.nseg > 1) {
+    k.xy_stages = 2;
+    k.dots = 0;
+    if (int rc = la_tc_launch<true, false>(k, roles, st)) return rc;
+    LaMmaFlags f = {};
+    f.all_segments = k.all_segments;
+    const int64_t elems = a.B * a.H * kTcDim * kTcDim;
+    if (elems / 256 > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
+    la_mma_join_kernel<kTcDim, kTcDim><<<dim3((unsigned)((elems + 255) / 256), roles), 256, 0, st>>>(a, f);
+    PTB_CUDA(cudaGetLastError());
+    for (int r = 0; r < roles; ++r)   // the segments' states are known: the update needs no float32 end any more
+      if (!a.p[r].dots) k.nu[r] = 2;
+  }
+  if (!dots) {
+    k.xy_stages = 2;
+    return la_tc_launch<false, false>(k, roles, st);
+  }
+  // the passes with dots, then the others (another use of the shared memory)
+  LaTcArgs part = k;
+  int with = 0, without = 0;
+  LaTcArgs plain = k;
+  for (int r = 0; r < roles; ++r) {
+    LaTcArgs& to = a.p[r].dots ? part : plain;
+    const int at = a.p[r].dots ? with++ : without++;
+    to.a.p[at] = a.p[r];
+    to.x[at] = k.x[r]; to.y[at] = k.y[r]; to.z[at] = k.z[r]; to.w[at] = k.w[r];
+    to.nu[at] = k.nu[r]; to.ns[at] = k.ns[r];
+  }
+  // entering states of segments are found by role: the passes with dots come first in the caller's order
+  plain.a.seg = k.a.seg + (int64_t)with * (a.nseg + 1) * a.B * a.H * a.seg_stride;
+  part.xy_stages = 1;
+  plain.xy_stages = 2;
+  if (int rc = la_tc_launch<false, true>(part, with, st)) return rc;
+  return without ? la_tc_launch<false, false>(plain, without, st) : PTB_OK;
+}
+
 template <class T, class S>
-static int la_run(LaArgs<S>& a, int roles, const LaPlan& l, void* ws, cudaStream_t st) {
+static int la_run(LaArgs<S>& a, LaTcArgs* k, LaPath path, int roles, const LaPlan& l, void* ws, uint32_t* status, cudaStream_t st) {
   la_workspace(a, l, ws);
-  if constexpr (kLaMma<T>) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    if (path == kLaTc) {
+      k->a = a;
+      k->status = status;
+      k->wait_cycles = (long long)(g_wait_ns * 2);   // SM clocks are below 2 GHz
+      return la_tc_run(*k, roles, st);
+    }
     bool dots = false;
     for (int r = 0; r < roles; ++r) dots = dots || a.p[r].dots;
     const bool vec = la_mma_vec(a, roles);
@@ -188,15 +302,20 @@ static int la_run(LaArgs<S>& a, int roles, const LaPlan& l, void* ws, cudaStream
   }
 }
 
+template <class T, class S>
+static LaPath la_path(LaTcArgs* k, const LaArgs<S>& a, int roles) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return la_tc_setup(k, a, roles) ? kLaTc : kLaMma;
+  return kLaSimt;
+}
+
 static void la_strides(int64_t (&d)[3], const int64_t* s) { for (int i = 0; i < 3; ++i) d[i] = s[i]; }
 
 template <class T, class S>
 static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs,
                   const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
                   const int64_t* gs, const int32_t* lengths, const void* init, double scale, void* o, void* fin,
-                  void* ws, int64_t wsb, cudaStream_t st) {
-  const LaPlan l = la_plan_of<T, S>({B, T_, H, Dk, Dv}, 1, false);
-  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total) return PTB_ERR_WORKSPACE;
+                  void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u)) return PTB_ERR_WORKSPACE;
   LaArgs<S> a = {};
   LaPass<S>& p = a.p[0];
   p.x = q; p.y = k; p.z = v;
@@ -210,7 +329,11 @@ static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
   la_strides(a.gs, gs);
   a.lengths = lengths;
   a.B = B; a.T = T_; a.H = H;
-  return la_run<T, S>(a, 1, l, ws, st);
+  LaTcArgs tc = {};
+  const LaPath path = la_path<T, S>(&tc, a, 1);
+  const LaPlan l = la_plan_of<S>(path, {B, T_, H, Dk, Dv}, 1, false);
+  if (wsb < l.total) return PTB_ERR_WORKSPACE;
+  return la_run<T, S>(a, &tc, path, 1, l, ws, status, st);
 }
 
 template <class T, class S>
@@ -218,10 +341,9 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
                   const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
                   const int64_t* gs, const int32_t* lengths, const void* init, double scale, const void* go,
                   const int64_t* gos, const void* gfin, void* gq, void* gk, void* gv, void* gg, int gg_per_token,
-                  void* ginit, void* ws, int64_t wsb, cudaStream_t st) {
+                  void* ginit, void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
   const bool dec = gg != nullptr;
-  const LaPlan l = la_plan_of<T, S>({B, T_, H, Dk, Dv}, 3, dec);
-  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total) return PTB_ERR_WORKSPACE;
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u)) return PTB_ERR_WORKSPACE;
   char* w = static_cast<char*>(ws);
   LaArgs<S> a = {};
   a.g = static_cast<const S*>(g);
@@ -237,7 +359,6 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
     p.init = static_cast<const S*>(init);
     p.M = (int)Dv; p.N = (int)Dk; p.state_t = 1;
     p.po = (S)scale; p.pz = (S)1;
-    if (dec) { p.bounds = reinterpret_cast<S*>(w + l.qb_off); p.dots = reinterpret_cast<S*>(w + l.qd_off); }
   }
   if (gk || dec || ginit) {
     LaPass<S>& p = a.p[roles++];
@@ -248,7 +369,6 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
     p.fin = static_cast<S*>(ginit);
     p.M = (int)Dv; p.N = (int)Dk; p.state_t = 1; p.reverse = 1;
     p.po = (S)1; p.pz = (S)scale;
-    if (dec) { p.bounds = reinterpret_cast<S*>(w + l.rb_off); p.dots = reinterpret_cast<S*>(w + l.kd_off); }
   }
   if (gv) {
     LaPass<S>& p = a.p[roles++];
@@ -260,22 +380,37 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
     p.po = (S)1; p.pz = (S)scale;
   }
   if (roles == 0) return PTB_OK;
-  if (int rc = la_run<T, S>(a, roles, l, ws, st)) return rc;
+  LaTcArgs tc = {};
+  const LaPath path = la_path<T, S>(&tc, a, roles);
+  const LaPlan l = la_plan_of<S>(path, {B, T_, H, Dk, Dv}, 3, dec);
+  if (wsb < l.total) return PTB_ERR_WORKSPACE;
+  if (dec) {   // the first two passes give what the gradient of the decays is made of
+    a.p[0].bounds = reinterpret_cast<S*>(w + l.qb_off);
+    a.p[0].dots = reinterpret_cast<S*>(w + l.qd_off);
+    a.p[1].bounds = reinterpret_cast<S*>(w + l.rb_off);
+    a.p[1].dots = reinterpret_cast<S*>(w + l.kd_off);
+  }
+  if (int rc = la_run<T, S>(a, &tc, path, roles, l, ws, status, st)) return rc;
   if (dec && l.nchunk > 0) {
     LaDecayArgs<S> d = {};
     d.s_bounds = reinterpret_cast<const S*>(w + l.qb_off);
     d.r_bounds = reinterpret_cast<const S*>(w + l.rb_off);
     d.qd = reinterpret_cast<const S*>(w + l.qd_off);
     d.kd = reinterpret_cast<const S*>(w + l.kd_off);
-    d.q_slices = d.k_slices = kLaMma<T> ? 1 : (int)((Dk + LaGeom<S>::NS - 1) / LaGeom<S>::NS);
+    const int width = path == kLaMma ? kLaMaxDim : path == kLaTc ? kTcSlice : LaGeom<S>::NS, slices = (int)((Dk + width - 1) / width);
+    d.q_slices = d.k_slices = path == kLaTc ? 2 * slices : slices;   // there two warps share a row
     d.g = a.g;
     la_strides(d.gs, gs);
     d.lengths = lengths;
     d.B = B; d.T = T_; d.H = H; d.MN = l.bound_elems;
+    d.used = path == kLaTc ? (int64_t)slices * kTcSlice * kTcDim : l.bound_elems;   // columns a pass had
     if (gg_per_token) d.dg = static_cast<S*>(gg);
     else d.part = reinterpret_cast<double*>(w + l.part_off);
     if (B * H * l.nchunk > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
-    la_decay_grad_kernel<S, kLaMma<T> ? kLaMmaChunk : LaGeom<S>::C><<<(unsigned)(B * H * l.nchunk), 256, 0, st>>>(d);
+    const unsigned grid = (unsigned)(B * H * l.nchunk);
+    if (path == kLaTc) la_decay_grad_kernel<S, kTcChunk><<<grid, 256, 0, st>>>(d);
+    else if (path == kLaMma) la_decay_grad_kernel<S, kLaMmaChunk><<<grid, 256, 0, st>>>(d);
+    else la_decay_grad_kernel<S, LaGeom<S>::C><<<grid, 256, 0, st>>>(d);
     PTB_CUDA(cudaGetLastError());
   }
   if (dec && !gg_per_token) {
@@ -332,7 +467,10 @@ int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, in
   if (la_check(dtype, B, T, H, Dk, Dv) != PTB_OK) return 0;
   const LaSize z = {B, T, H, Dk, Dv};
   const int roles = backward ? 3 : 1;
-  PTB_LA_TYPES((la_plan_of<T_, S_>(z, roles, decay_grad).total))
+  if (dtype == PTB_F64) return la_plan_of<double>(kLaSimt, z, roles, decay_grad).total;
+  if (dtype != PTB_BF16) return la_plan_of<float>(kLaSimt, z, roles, decay_grad).total;
+  // which of the tensor-core kernels run depends on the operands' alignment too: room for either
+  return std::max(la_mma_plan(z, roles, decay_grad).total, la_tc_plan(z, roles, decay_grad).total);
 }
 
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
@@ -340,12 +478,11 @@ int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
                              const int32_t* lengths, const void* init, double scale, void* o, void* fin,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
-  (void)status;
   if (int rc = la_check(dtype, B, T, H, Dk, Dv)) return rc;
   if (B == 0 || H == 0) return PTB_OK;
   if ((T > 0 && (!q || !k || !v || !o || !log_decay)) || !q_strides || !k_strides || !v_strides || !log_decay_strides) return PTB_ERR_ARG;
   PTB_LA_TYPES((la_fwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
-                               lengths, init, scale, o, fin, workspace, workspace_bytes, (cudaStream_t)stream)))
+                               lengths, init, scale, o, fin, workspace, workspace_bytes, status, (cudaStream_t)stream)))
 }
 
 int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
@@ -355,7 +492,6 @@ int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t
                              const int64_t* grad_o_strides, const void* grad_fin, void* grad_q, void* grad_k,
                              void* grad_v, void* grad_log_decay, int grad_log_decay_per_token, void* grad_init,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
-  (void)status;
   if (int rc = la_check(dtype, B, T, H, Dk, Dv)) return rc;
   if (B == 0 || H == 0) return PTB_OK;
   if ((T > 0 && (!q || !k || !v || !log_decay || !grad_o)) || !q_strides || !k_strides || !v_strides || !log_decay_strides ||
@@ -364,7 +500,7 @@ int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t
   PTB_LA_TYPES((la_bwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
                                lengths, init, scale, grad_o, grad_o_strides, grad_fin, grad_q, grad_k, grad_v,
                                grad_log_decay, grad_log_decay_per_token, grad_init, workspace, workspace_bytes,
-                               (cudaStream_t)stream)))
+                               status, (cudaStream_t)stream)))
 }
 
 int ptb_linear_attention_step(int dtype, int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q,

@@ -370,7 +370,7 @@ struct LaDecayArgs {
   const S* g;
   int64_t gs[3];
   const int32_t* lengths;
-  int64_t B, T, H, MN;
+  int64_t B, T, H, MN, used;      // scalars between two states, and how many of them count
   S* dg;           // (B,T,H), or NULL
   double* part;    // [chunk][bh] sums over a chunk, or NULL
 };
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(256) la_decay_grad_kernel(const LaDecayArgs<S>
   if (n > 0) {
     const S* s = a.s_bounds + (bh * nchunk + c) * a.MN;
     const S* r = a.r_bounds + (bh * nchunk + c) * a.MN;
-    for (int64_t i = tid; i < a.MN; i += 256) acc += (double)s[i] * (double)r[i];
+    for (int64_t i = tid; i < a.used; i += 256) acc += (double)s[i] * (double)r[i];
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) acc += __shfl_down_sync(0xffffffffu, acc, d);

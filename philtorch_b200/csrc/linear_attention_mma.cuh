@@ -89,7 +89,7 @@ template <int MP, int NP, bool VEC, bool STATES_ONLY>
 __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, const LaMmaFlags f) {
   using Sm = LaMmaSmem<MP, NP>;
   constexpr int C = kLaMmaChunk, MT = MP / 8, NJ = NP / 64;   // 8-wide tiles of m; 16-high tiles of n per warp
-  extern __shared__ __align__(128) unsigned char la_smem[];
+  extern __shared__ __align__(128) unsigned char la_mma_smem[];
   const int role = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
   const LaPass<float>& p = a.p[role];
   if (STATES_ONLY && f.all_segments && !p.fin && blockIdx.x % a.nseg == a.nseg - 1) return;   // nobody asks for its end
@@ -109,8 +109,8 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(p.w) + b * p.ws[0] + h * p.ws[2];
   const float* g = a.g + b * a.gs[0] + h * a.gs[2];
 
-  unsigned char* const misc = la_smem + f.stages * Sm::STAGE + (dots ? Sm::Z : 0);
-  unsigned char* const wt_ptr = la_smem + f.stages * Sm::STAGE;
+  unsigned char* const misc = la_mma_smem + f.stages * Sm::STAGE + (dots ? Sm::Z : 0);
+  unsigned char* const wt_ptr = la_mma_smem + f.stages * Sm::STAGE;
   const uint32_t s_w = smem_u32(wt_ptr), s_p = smem_u32(misc);
   double* const G = reinterpret_cast<double*>(misc + Sm::P);
   float* const win = reinterpret_cast<float*>(G + C);
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
   auto fetch = [&](int64_t ci, int stage) {
     const int64_t c = chunk_of(ci), t0 = c * C;
     const int n = valid(c);
-    unsigned char* sp = la_smem + stage * Sm::STAGE;
+    unsigned char* sp = la_mma_smem + stage * Sm::STAGE;
     const uint32_t sx = smem_u32(sp);
     if (n > 0) {
       if (!STATES_ONLY) la_tile_load<MP, VEC>(sx, sp, x, p.xs[1], t0, n, M, tid);
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
       else la_cp_wait<0>();
     }
     __syncthreads();
-    const uint32_t sx = smem_u32(la_smem + stage * Sm::STAGE), sy = sx + Sm::X, sz = sy + Sm::X;
+    const uint32_t sx = smem_u32(la_mma_smem + stage * Sm::STAGE), sy = sx + Sm::X, sz = sy + Sm::X;
     const double E = G[C - 1];
 
     if constexpr (!STATES_ONLY) {
