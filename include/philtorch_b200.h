@@ -503,7 +503,7 @@ int ptb_modal_bank_bwd(int dtype, int64_t rows, int64_t M, int64_t N, const void
  * 0..T: tokens from lengths[b] on are not read, leave the state alone and give zeros.  init, fin: optional dense
  * (B,H,Dk,Dv), the state before the first and after the last token.  o: dense (B,T,H,Dv).
  * workspace: ptb_linear_attention_workspace_bytes(..., backward, decay_grad) bytes, 256-byte aligned, private to the
- * call until it completes.  status is not used (no kernel here waits on another CTA); it may be NULL. */
+ * call until it completes; none (NULL) where that is 0.  status: as above (waits inside a CTA are bounded). */
 int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
                                              int backward, int decay_grad);
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,

@@ -242,9 +242,25 @@ _current_device = torch._C._cuda_getDevice                # both skip the Python
 _current_raw_stream = torch._C._cuda_getCurrentRawStream  # this function runs once per kernel launch
 
 
+def eager(t: torch.Tensor) -> bool:
+    """Whether an op may be run by calling its implementation: a plain tensor, and nobody (a compiler, a
+    dispatch mode, a functional transform) watching the dispatcher."""
+    return (type(t) in _PLAIN and t.is_cuda and not torch.compiler.is_compiling() and not _dispatch_modes()
+            and _transforms() is None)
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_transforms = torch._C._functorch.peek_interpreter_stack
+
+
 def call(fn, device: torch.device, B: int, T: int, *args, ws_bytes: int = -1) -> None:
     """Runs ``fn(*args, workspace, bytes, status, stream)`` on ``device``'s current stream."""
-    ws = workspace(B, T, device) if ws_bytes < 0 else torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    if ws_bytes:
+        ws = workspace(B, T, device) if ws_bytes < 0 else torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+        at, size = ws.data_ptr(), ws.numel()
+    else:
+        at, size = None, 0
     idx = device.index
     if idx is None:
         idx = _current_device()
@@ -253,9 +269,9 @@ def call(fn, device: torch.device, B: int, T: int, *args, ws_bytes: int = -1) ->
         st = status_word(device)
     if idx != _current_device():
         with torch.cuda.device(idx):
-            rc = fn(*args, ws.data_ptr(), ws.numel(), st.data_ptr(), _current_raw_stream(idx))
+            rc = fn(*args, at, size, st.data_ptr(), _current_raw_stream(idx))
     else:
-        rc = fn(*args, ws.data_ptr(), ws.numel(), st.data_ptr(), _current_raw_stream(idx))
+        rc = fn(*args, at, size, st.data_ptr(), _current_raw_stream(idx))
     if rc != 0:
         check(rc, fn.__name__)
     if CHECK_EVERY_CALL:

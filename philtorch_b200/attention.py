@@ -37,6 +37,16 @@ def state_dtype(dtype: torch.dtype) -> torch.dtype:
     return torch.float64 if dtype == torch.float64 else torch.float32
 
 
+def _strides3(t: Tensor):
+    a, b, c, _ = t.stride()
+    return _I3(a, b, c)
+
+
+def _strides2(t: Tensor):
+    a, b, _ = t.stride()
+    return _I2(a, b)
+
+
 def _rows(t: Tensor) -> Tensor:
     """The tensor with its last axis dense; the other strides are the kernels' arguments (views of one fused
     projection, or heads shared through ``expand``, are read in place)."""
@@ -52,6 +62,13 @@ def _code(t: Tensor) -> int:
 
 
 def _check(q: Tensor, k: Tensor, v: Tensor, g: Tensor, init: Optional[Tensor], lengths: Optional[Tensor]) -> None:
+    # the common case in one expression: the explanations below cost more host time than the launch
+    shape, dt = q.shape, q.dtype
+    if (len(shape) == 4 and k.shape == shape and v.dim() == 4 and v.shape[:3] == shape[:3] and k.dtype == dt and v.dtype == dt
+            and 1 <= shape[3] <= MAX_HEAD_DIM and 1 <= v.shape[3] <= MAX_HEAD_DIM and lengths is None
+            and g.dtype == state_dtype(dt) and (g.shape == shape[2:3] or g.shape == shape[:3])
+            and (init is None or (init.dtype == g.dtype and init.shape == (shape[0], shape[2], shape[3], v.shape[3])))):
+        return
     torch._check(q.dim() == 4, lambda: f"q must be 4D (batch, time, heads, Dk), got {tuple(q.shape)}")
     torch._check(k.shape == q.shape, lambda: f"k must have the shape of q, got {tuple(k.shape)} and {tuple(q.shape)}")
     torch._check(v.dim() == 4 and v.shape[:3] == q.shape[:3],
@@ -78,10 +95,6 @@ def _check(q: Tensor, k: Tensor, v: Tensor, g: Tensor, init: Optional[Tensor], l
 
 def _decay_strides(g: Tensor):
     return _I3(0, 0, g.stride(0)) if g.dim() == 1 else _I3(*g.stride())
-
-
-def _strides(t: Tensor):
-    return _I3(*t.stride()[:3])
 
 
 _ws_bytes: dict = {}
@@ -127,8 +140,8 @@ def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state):
     o = v.new_empty((B, T, H, Dv))
     state = log_decay.new_empty((B, H, Dk, Dv) if want_state else (0,))
     if B and H and (T or want_state):
-        _lib.call(lib.ptb_linear_attention_fwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides(q), ptr(k), _strides(k),
-                  ptr(v), _strides(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(o),
+        _lib.call(lib.ptb_linear_attention_fwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides3(q), ptr(k), _strides3(k),
+                  ptr(v), _strides3(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(o),
                   ptr(state) if want_state else None, ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 0, 0))
     return o, state
 
@@ -150,9 +163,9 @@ def _linear_attention_bwd(q, k, v, log_decay, init, lengths, scale, grad_o, grad
     ginit = log_decay.new_empty((B, H, Dk, Dv) if need_init else (0,))
     if B and H:
         opt = lambda t, need: ptr(t) if need else None   # noqa: E731
-        _lib.call(lib.ptb_linear_attention_bwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides(q), ptr(k), _strides(k),
-                  ptr(v), _strides(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(grad_o),
-                  _strides(grad_o), ptr(grad_state), opt(gq, need_q), opt(gk, need_k), opt(gv, need_v),
+        _lib.call(lib.ptb_linear_attention_bwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides3(q), ptr(k), _strides3(k),
+                  ptr(v), _strides3(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(grad_o),
+                  _strides3(grad_o), ptr(grad_state), opt(gq, need_q), opt(gk, need_k), opt(gv, need_v),
                   opt(gg, need_decay), int(log_decay.dim() == 3), opt(ginit, need_init),
                   ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 1, int(need_decay)))
     else:
@@ -161,6 +174,12 @@ def _linear_attention_bwd(q, k, v, log_decay, init, lengths, scale, grad_o, grad
 
 
 def _check_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, state: Tensor) -> None:
+    shape, dt = q.shape, q.dtype
+    if (len(shape) == 3 and k.shape == shape and v.dim() == 3 and v.shape[:2] == shape[:2] and k.dtype == dt and v.dtype == dt
+            and 1 <= shape[2] <= MAX_HEAD_DIM and 1 <= v.shape[2] <= MAX_HEAD_DIM and g.dtype == state_dtype(dt)
+            and (g.shape == shape[1:2] or g.shape == shape[:2]) and state.dtype == g.dtype
+            and state.shape == (shape[0], shape[1], shape[2], v.shape[2]) and state.is_contiguous()):
+        return
     torch._check(q.dim() == 3, lambda: f"q must be 3D (batch, heads, Dk), got {tuple(q.shape)}")
     torch._check(k.shape == q.shape, lambda: f"k must have the shape of q, got {tuple(k.shape)} and {tuple(q.shape)}")
     torch._check(v.dim() == 3 and v.shape[:2] == q.shape[:2],
@@ -196,8 +215,8 @@ def _linear_attention_step(q, k, v, log_decay, state, scale):
     o = v.new_empty((B, H, Dv))
     if B and H:
         gs = _I2(0, log_decay.stride(0)) if log_decay.dim() == 1 else _I2(*log_decay.stride())
-        _lib.launch(lib.ptb_linear_attention_step, dev, _code(q), B, H, Dk, Dv, ptr(q), _I2(*q.stride()[:2]), ptr(k),
-                    _I2(*k.stride()[:2]), ptr(v), _I2(*v.stride()[:2]), ptr(log_decay), gs, scale, ptr(state),
+        _lib.launch(lib.ptb_linear_attention_step, dev, _code(q), B, H, Dk, Dv, ptr(q), _strides2(q), ptr(k),
+                    _strides2(k), ptr(v), _strides2(v), ptr(log_decay), gs, scale, ptr(state),
                     _I2(*state.stride()[:2]), ptr(o))
         torch.autograd.graph.increment_version(state)
     return o
@@ -233,13 +252,33 @@ _ops = torch.ops.philtorch_b200
 
 
 # ------------------------------------------------------------------------------------------------ autograd
+def _forward(q, k, v, log_decay, init, lengths, scale, want_state):
+    if q.device.type == "cpu":
+        _lib.require_cuda(q)
+    run = _linear_attention if _lib.eager(q) else _ops.linear_attention
+    return run(q, k, v, log_decay, init, lengths, scale, want_state)
+
+
+def _backward(ctx: Any, grad_o: Optional[Tensor], grad_state: Optional[Tensor]):
+    need = ctx.needs_input_grad[:5]
+    if (grad_o is None and grad_state is None) or not any(need):
+        return (None,) * 8
+    q, k, v, log_decay, init, lengths = ctx.saved_tensors
+    run = _linear_attention_bwd if _lib.eager(q) else _ops.linear_attention_bwd
+    grads = run(q, k, v, log_decay, init, lengths, ctx.scale, grad_o, grad_state, *need)
+    return (*(g if n else None for g, n in zip(grads, need)), None, None, None)
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class LinearAttention(Function):
     """(q, k, v, log_decay, init or None, lengths or None, scale, want_state) -> (o, final state).  First
     derivatives; the backward pass recomputes the states instead of keeping them."""
 
     @staticmethod
     def forward(ctx: Any, q, k, v, log_decay, init, lengths, scale: float, want_state: bool):
-        o, state = _ops.linear_attention(q, k, v, log_decay, init, lengths, scale, want_state)
+        o, state = _forward(q, k, v, log_decay, init, lengths, scale, want_state)
         ctx.save_for_backward(q, k, v, log_decay, init, lengths)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
@@ -248,14 +287,9 @@ class LinearAttention(Function):
         return o, state
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad_o: Optional[Tensor], grad_state: Optional[Tensor]):
-        need = ctx.needs_input_grad[:5]
-        if (grad_o is None and grad_state is None) or not any(need):
-            return (None,) * 8
-        q, k, v, log_decay, init, lengths = ctx.saved_tensors
-        grads = _ops.linear_attention_bwd(q, k, v, log_decay, init, lengths, ctx.scale, grad_o, grad_state, *need)
-        return (*(g if n else None for g, n in zip(grads, need)), None, None, None)
+        # (the guard against second derivatives is only needed, and only paid, where a graph is being recorded)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_o, grad_state)
 
 
 def _normalised(o: Tensor, eps: Optional[float], weight: Optional[Tensor], bias: Optional[Tensor]) -> Tensor:
@@ -271,21 +305,26 @@ def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tens
            lengths: Optional[Tensor], return_state: Optional[bool], norm_eps: Optional[float],
            norm_weight: Optional[Tensor], norm_bias: Optional[Tensor]):
     want = (zi is not None) if return_state is None else bool(return_state)
-    _lib.require_cuda(q, k, v, log_decay, zi, lengths)
-    tensors = (q, k, v, log_decay, zi)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or (zi is not None and zi.requires_grad)):
         o, state = LinearAttention.apply(q, k, v, log_decay, zi, lengths, float(scale), want)
     else:
-        o, state = _ops.linear_attention(q, k, v, log_decay, zi, lengths, float(scale), want)
-    o = _normalised(o, norm_eps, norm_weight, norm_bias)
+        o, state = _forward(q, k, v, log_decay, zi, lengths, float(scale), want)
+    if norm_eps is not None or norm_weight is not None or norm_bias is not None:
+        o = _normalised(o, norm_eps, norm_weight, norm_bias)
     return (o, state) if want else o
 
 
 def attend_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, scale: float,
                 norm_eps: Optional[float], norm_weight: Optional[Tensor], norm_bias: Optional[Tensor]) -> Tensor:
-    _lib.require_cuda(q, k, v, log_decay, state)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or state.requires_grad):
         raise RuntimeError("linear_attention_step updates its state in place and is not differentiable: call it under "
                            "torch.no_grad(), or linear_attention for gradients")
-    o = _ops.linear_attention_step(q, k, v, log_decay, state, float(scale))
-    return _normalised(o, norm_eps, norm_weight, norm_bias)
+    if q.device.type == "cpu":
+        _lib.require_cuda(q)
+    run = _linear_attention_step if _lib.eager(q) else _ops.linear_attention_step
+    o = run(q, k, v, log_decay, state, float(scale))
+    if norm_eps is not None or norm_weight is not None or norm_bias is not None:
+        o = _normalised(o, norm_eps, norm_weight, norm_bias)
+    return o

@@ -18,13 +18,12 @@ struct LaPlan {
 };
 
 // Few (batch, head) pairs: the time axis is cut into segments that run side by side.  Their entering states
-// come from a first pass that only forms the states (it reads two of the three operands), so a cut pays
-// where it at least halves the rows each CTA walks; a segment keeps at least 8 chunks.
+// come from a first pass that only forms states (about half the work of a chunk), so a cut into n segments takes
+// about 1.5 / n of the time plus two launches: it pays from n = 2 on, where the row has chunks to spare.
 static void la_cut(int64_t ctas, int64_t nchunk, int64_t room, int* nseg, int* seg_chunks) {
-  int64_t n = ctas > 0 ? room / ctas : 1;
-  n = std::min(n, nchunk / 8);
-  if (n < 3) n = 1;
-  int64_t per = n > 1 ? (nchunk + n - 1) / n : std::max<int64_t>(nchunk, 1);
+  int64_t n = ctas > 0 ? std::min(room / ctas, nchunk / 2) : 1;
+  if (n < 2 || nchunk < 8) n = 1;
+  const int64_t per = n > 1 ? (nchunk + n - 1) / n : std::max<int64_t>(nchunk, 1);
   *seg_chunks = (int)per;
   *nseg = n > 1 ? (int)((nchunk + per - 1) / per) : 1;
 }
@@ -51,7 +50,7 @@ static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int sl
   l.qd_off = take(decay_grad ? 2 * l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
   l.kd_off = take(decay_grad ? 2 * l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
   l.part_off = take(decay_grad ? BH * l.nchunk * sizeof(double) : 0);
-  l.total = std::max<int64_t>(at, 256);
+  l.total = at;
   return l;
 }
 template <class S>
@@ -315,7 +314,6 @@ static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
                   const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
                   const int64_t* gs, const int32_t* lengths, const void* init, double scale, void* o, void* fin,
                   void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
-  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u)) return PTB_ERR_WORKSPACE;
   LaArgs<S> a = {};
   LaPass<S>& p = a.p[0];
   p.x = q; p.y = k; p.z = v;
@@ -332,7 +330,7 @@ static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
   LaTcArgs tc = {};
   const LaPath path = la_path<T, S>(&tc, a, 1);
   const LaPlan l = la_plan_of<S>(path, {B, T_, H, Dk, Dv}, 1, false);
-  if (wsb < l.total) return PTB_ERR_WORKSPACE;
+  if (l.total && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total)) return PTB_ERR_WORKSPACE;
   return la_run<T, S>(a, &tc, path, 1, l, ws, status, st);
 }
 
@@ -343,7 +341,6 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
                   const int64_t* gos, const void* gfin, void* gq, void* gk, void* gv, void* gg, int gg_per_token,
                   void* ginit, void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
   const bool dec = gg != nullptr;
-  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u)) return PTB_ERR_WORKSPACE;
   char* w = static_cast<char*>(ws);
   LaArgs<S> a = {};
   a.g = static_cast<const S*>(g);
@@ -383,7 +380,7 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
   LaTcArgs tc = {};
   const LaPath path = la_path<T, S>(&tc, a, roles);
   const LaPlan l = la_plan_of<S>(path, {B, T_, H, Dk, Dv}, 3, dec);
-  if (wsb < l.total) return PTB_ERR_WORKSPACE;
+  if (l.total && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total)) return PTB_ERR_WORKSPACE;
   if (dec) {   // the first two passes give what the gradient of the decays is made of
     a.p[0].bounds = reinterpret_cast<S*>(w + l.qb_off);
     a.p[0].dots = reinterpret_cast<S*>(w + l.qd_off);

@@ -12,25 +12,38 @@ static int ln_lanes(int width, int V) {
   return 1024;
 }
 
-// CTAs over the rows in the backward kernel; each leaves one partial row of the parameter gradients, so
-// there are no more of them than fill the machine
-static int64_t ln_row_blocks(int64_t rows, int groups, int L) {
-  const int slots = L > 256 ? 1 : 256 / L;
-  const int64_t per_sm = L > 256 ? 1 : 2;
+// CTAs over the rows.  Backward: each leaves one partial row of the parameter gradients, so there are no more of
+// them than are resident at once; forward: a few rounds of them, so that the last round is short
+static int64_t ln_row_blocks(int64_t rows, int groups, int L, int64_t per_sm) {
+  const int slots = ln_threads(L) / L;
   const int64_t want = std::max<int64_t>(1, (kLnSms * per_sm + groups - 1) / groups);
   return std::max<int64_t>(1, std::min<int64_t>(want, (rows + slots - 1) / slots));
 }
+static int64_t ln_bwd_blocks(int64_t rows, int groups, int L) { return ln_row_blocks(rows, groups, L, L > 256 ? 1 : 2); }
 
 template <class T, class S, int V, int L, int NV>
 static int ln_launch(const LnArgs<S>& a, bool bwd, int64_t blocks, cudaStream_t st) {
-  constexpr int NT = L > 256 ? L : 256, SLOTS = NT / L;
+  constexpr int NT = ln_threads(L), SLOTS = NT / L;
+  constexpr int kPipe = ln_pipe_bytes<T, S, V, L, NV>(1), kPipeBwd = ln_pipe_bytes<T, S, V, L, NV>(2);
+  static bool ready[kMaxDevices] = {};
+  int dev = 0;
+  PTB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return PTB_ERR_ARG;
+  {
+    std::lock_guard<std::mutex> lock(init_mutex());
+    if (!ready[dev]) {
+      PTB_CUDA(cudaFuncSetAttribute(ln_fwd_kernel<T, S, V, L, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPipe));
+      PTB_CUDA(cudaFuncSetAttribute(ln_bwd_kernel<T, S, V, L, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    std::max(kPipeBwd, 48 * 1024)));
+      ready[dev] = true;
+    }
+  }
   if (!bwd) {
-    const int64_t units = a.rows * a.groups, need = (units + SLOTS - 1) / SLOTS;
-    const int64_t grid = std::min<int64_t>(need, (int64_t)kLnSms * 2048 / NT * 4);
-    ln_fwd_kernel<T, S, V, L, NV><<<(unsigned)grid, NT, 0, st>>>(a);
+    const int64_t grid = ln_row_blocks(a.rows, a.groups, L, 8);
+    ln_fwd_kernel<T, S, V, L, NV><<<dim3((unsigned)grid, a.groups), NT, kPipe, st>>>(a);
   } else {
-    const int smem = SLOTS > 1 ? SLOTS * a.width * (int)sizeof(S) : 0;   // at most 256 * V * NV scalars = 32 KB
-    ln_bwd_kernel<T, S, V, L, NV><<<dim3((unsigned)blocks, a.groups), NT, smem, st>>>(a);
+    const int join = SLOTS > 1 ? SLOTS * a.width * (int)sizeof(S) : 0;   // at most 256 * V * NV scalars = 32 KB
+    ln_bwd_kernel<T, S, V, L, NV><<<dim3((unsigned)blocks, a.groups), NT, std::max(kPipeBwd, join), st>>>(a);
   }
   PTB_CUDA(cudaGetLastError());
   return PTB_OK;
@@ -68,7 +81,7 @@ template <class T, class S>
 static int ln_bwd(LnArgs<S>& a, void* gw, void* gb, void* ws, int64_t wsb, cudaStream_t st) {
   const int V = ln_vec<T, S>(a);
   const int64_t C = (int64_t)a.groups * a.width;
-  const int64_t blocks = ln_row_blocks(a.rows, a.groups, ln_lanes(a.width, V));
+  const int64_t blocks = ln_bwd_blocks(a.rows, a.groups, ln_lanes(a.width, V));
   const int64_t one = align_up(blocks * C * (int64_t)sizeof(S), 256), need = (gw ? one : 0) + (gb ? one : 0);
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < need)) return PTB_ERR_WORKSPACE;
   char* w = static_cast<char*>(ws);
@@ -95,6 +108,7 @@ static LnArgs<S> ln_args(int64_t rows, int64_t groups, int64_t width, const void
   LnArgs<S> a = {};
   a.x = x; a.x_stride = x_stride;
   a.w = w; a.b = b; a.w_wide = w_wide;
+  a.w_vec = aligned16(w) && aligned16(b);
   a.mean = static_cast<S*>(mean); a.rstd = static_cast<S*>(rstd);
   a.rows = rows; a.groups = (int)groups; a.width = (int)width;
   return a;
@@ -118,7 +132,7 @@ int64_t ptb_layer_norm_bwd_workspace_bytes(int dtype, int64_t rows, int64_t grou
   if (ln_check(dtype, rows, groups, width) != PTB_OK) return 0;
   const int64_t s = dtype == PTB_F64 ? 8 : 4, vec = dtype == PTB_F64 ? 2 : dtype == PTB_F32 ? 4 : 8;
   int64_t most = 1;   // the pointers' alignment may rule the wide accesses out: room for either choice
-  for (int V : {1, (int)vec}) most = std::max(most, ln_row_blocks(rows, (int)groups, ln_lanes((int)width, V)));
+  for (int V : {1, (int)vec}) most = std::max(most, ln_bwd_blocks(rows, (int)groups, ln_lanes((int)width, V)));
   return 2 * align_up(most * groups * width * s, 256);
 }
 

@@ -429,14 +429,22 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
           la_ldm_t(bv, la_at<MP>(sy, 16 * kk + (lane & 7) + (((lane >> 3) & 1) << 3), 2 * q + (lane >> 4)));
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
-            if (acc_u) {   // smallest first
-              la_mma(st[j][2 * q], t2v[j], bv[0], bv[1]);
-              la_mma(st[j][2 * q + 1], t2v[j], bv[2], bv[3]);
+            // terms added up on their own, smallest first, then to the state: the tensor core's additions truncate, which
+            // against the whole state would add up over the chunks
+            float u0[4] = {}, u1[4] = {};
+            if (acc_u) {
+              la_mma(u0, t2v[j], bv[0], bv[1]);
+              la_mma(u1, t2v[j], bv[2], bv[3]);
             }
-            la_mma(st[j][2 * q], t1v[j], bv[0], bv[1]);
-            la_mma(st[j][2 * q + 1], t1v[j], bv[2], bv[3]);
-            la_mma(st[j][2 * q], t0v[j], bv[0], bv[1]);
-            la_mma(st[j][2 * q + 1], t0v[j], bv[2], bv[3]);
+            la_mma(u0, t1v[j], bv[0], bv[1]);
+            la_mma(u1, t1v[j], bv[2], bv[3]);
+            la_mma(u0, t0v[j], bv[0], bv[1]);
+            la_mma(u1, t0v[j], bv[2], bv[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              st[j][2 * q][e] += u0[e];
+              st[j][2 * q + 1][e] += u1[e];
+            }
           }
         }
       }

@@ -16,6 +16,7 @@
 // pairs inside a chunk from the float32 scores themselves.
 #pragma once
 #include "linear_attention_mma.cuh"
+#include "packed.cuh"
 #include "tensor_map.cuh"
 
 namespace ptb {
@@ -114,43 +115,14 @@ __device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap* map, int
       : "memory");
 }
 
-// pairs of float32 in one instruction
-__device__ __forceinline__ uint64_t tc_pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t tc_pair(uint32_t a, uint32_t b) { return tc_pair(__uint_as_float(a), __uint_as_float(b)); }
-__device__ __forceinline__ float2 tc_unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t tc_mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t tc_sub2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t tc_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint32_t tc_pack(uint64_t v) {   // two bfloat16
-  const float2 f = tc_unpair(v);
+using TcPair = Pair<float>;
+__device__ __forceinline__ TcPair tc_pair(uint32_t a, uint32_t b) { return TcPair(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ TcPair tc_pair(float a, float b) { return TcPair(a, b); }
+__device__ __forceinline__ uint32_t tc_pack(TcPair v) {   // two bfloat16
+  const float2 f = v.get();
   return la_pack(f.x, f.y);
 }
-__device__ __forceinline__ uint64_t tc_widen(uint32_t v) { return tc_pair(la_lo(v), la_hi(v)); }
+__device__ __forceinline__ TcPair tc_widen(uint32_t v) { return tc_pair(la_lo(v), la_hi(v)); }
 __device__ __forceinline__ bool tc_elect() {
   uint32_t on;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
@@ -456,7 +428,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         const int64_t c = chunk_of(i), t0 = c * C;
         const int n = valid(c), sz = i & 1;
         const float* const G = Gs + (i & 1) * 2 * C;
-        const uint64_t own_hi = tc_pair(row_own.x, row_own.x), own_lo = tc_pair(row_own.y, row_own.y);
+        const TcPair own_hi = tc_pair(row_own.x, row_own.x), own_lo = tc_pair(row_own.y, row_own.y);
         const float mine = row_mine, win = row_win, mid1 = row_mid1, mid2 = row_mid2;
         asm volatile("bar.sync 1, 256;" ::: "memory");   // every row's factors are written
         wait_warp(b_sc, i & 1);
@@ -474,21 +446,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
             const uint32_t on = pairs >> ((q & 1) * 16);
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-              const uint64_t d = tc_add2(tc_sub2(own_hi, *reinterpret_cast<const uint64_t*>(G + q * 16 + j)),
-                                         tc_sub2(own_lo, *reinterpret_cast<const uint64_t*>(G + C + q * 16 + j)));
-              const float2 e = tc_unpair(d);
-              const float2 w = tc_unpair(tc_mul2(tc_pair(v[j], v[j + 1]), tc_pair(tc_exp2(e.x), tc_exp2(e.y))));
+              const float2 e = ((own_hi - TcPair(*reinterpret_cast<const uint64_t*>(G + q * 16 + j))) +
+                                (own_lo - TcPair(*reinterpret_cast<const uint64_t*>(G + C + q * 16 + j)))).get();
+              const float2 w = (tc_pair(v[j], v[j + 1]) * tc_pair(tc_exp2(e.x), tc_exp2(e.y))).get();
               v[j] = on >> j & 1 ? __float_as_uint(w.x) : 0u;
               v[j + 1] = on >> (j + 1) & 1 ? __float_as_uint(w.y) : 0u;
             }
           } else {
             const int between = (rev ? (q >> 1) - quad : quad - (q >> 1)) - 1;
             const float from1 = mine * (between == 0 ? 1.f : between == 1 ? mid1 : mid2);
-            const uint64_t from = tc_pair(from1, from1);
+            const TcPair from(from1, from1);
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-              const uint64_t c2 = *reinterpret_cast<const uint64_t*>(cs + q * 16 + j);
-              const float2 w = tc_unpair(tc_mul2(tc_pair(v[j], v[j + 1]), tc_mul2(from, c2)));
+              const TcPair c2(*reinterpret_cast<const uint64_t*>(cs + q * 16 + j));
+              const float2 w = (tc_pair(v[j], v[j + 1]) * (from * c2)).get();
               v[j] = __float_as_uint(w.x);
               v[j + 1] = __float_as_uint(w.y);
             }
@@ -518,8 +489,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         tc_after();
         const int64_t t = t0 + row;
         __nv_bfloat16* const dst = o ? o + ((b * a.T + t) * a.H + h) * N + n0 : nullptr;
-        uint64_t ext = 0;
-        const uint64_t win2 = tc_pair(win, win), scale2 = tc_pair(scale_in, scale_in);
+        TcPair ext(0.f, 0.f);
+        const TcPair win2(win, win), scale2(scale_in, scale_in);
         uint32_t vi[2][16], vo[2][16];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -533,17 +504,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         for (int q = 0; q < 2; ++q) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint64_t r[4];
+            TcPair r[4];
             const int piece = 2 * (2 * part + q) + e;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = tc_mul2(tc_pair(vi[q][e * 8 + 2 * j], vi[q][e * 8 + 2 * j + 1]), win2);
+            for (int j = 0; j < 4; ++j) r[j] = tc_pair(vi[q][e * 8 + 2 * j], vi[q][e * 8 + 2 * j + 1]) * win2;
             if (DOTS) {
               const uint4 wv = *reinterpret_cast<const uint4*>(tc_smem + L.z + (sz * 2 + 1) * kTcPanel + row * 128 +
                                                               ((piece ^ (row & 7)) << 4));
-              ext = tc_fma2(r[0], tc_widen(wv.x), tc_fma2(r[1], tc_widen(wv.y), tc_fma2(r[2], tc_widen(wv.z), tc_fma2(r[3], tc_widen(wv.w), ext))));
+              ext = fma2(r[0], tc_widen(wv.x), fma2(r[1], tc_widen(wv.y), fma2(r[2], tc_widen(wv.z), fma2(r[3], tc_widen(wv.w), ext))));
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = tc_fma2(tc_pair(vo[q][e * 8 + 2 * j], vo[q][e * 8 + 2 * j + 1]), scale2, r[j]);
+            for (int j = 0; j < 4; ++j) r[j] = fma2(tc_pair(vo[q][e * 8 + 2 * j], vo[q][e * 8 + 2 * j + 1]), scale2, r[j]);
             uint4 pk = make_uint4(tc_pack(r[0]), tc_pack(r[1]), tc_pack(r[2]), tc_pack(r[3]));
             if (row >= n) pk = make_uint4(0, 0, 0, 0);
             if (dst && t < a.T && n0 + piece * 8 < N) *reinterpret_cast<uint4*>(dst + piece * 8) = pk;
@@ -553,7 +524,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
           arrive_warp(zw_empty + sz);
           if (row < n) {
             float2* d = reinterpret_cast<float2*>(p.dots + ((((int64_t)slice * 2 + part) * BH + bh) * a.T + t) * 2);
-            const float2 e = tc_unpair(ext);
+            const float2 e = ext.get();
             *d = make_float2(rowsum * scale_in, e.x + e.y);
           }
         }
@@ -599,7 +570,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     };
     if (count > 0) decays(0);
     auto advance = [&](int i) {   // S <- exp(E) S + U of chunk i
-      const uint64_t dec_hi = tc_pair(dec.x, dec.x), dec_lo = tc_pair(dec.y, dec.y);
+      const TcPair dec_hi(dec.x, dec.x), dec_lo(dec.y, dec.y);
       wait_warp(b_u, i & 1);
       tc_after();
 #pragma unroll
@@ -614,13 +585,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         tc_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          uint64_t v = tc_pair(u[j], u[j + 1]);
+          TcPair v = tc_pair(u[j], u[j + 1]);
           if (!DOTS) {
-            if (nu == 3) v = tc_add2(v, tc_add2(tc_pair(u1[j], u1[j + 1]), tc_pair(u2[j], u2[j + 1])));
-            else v = tc_add2(v, tc_pair(u1[j], u1[j + 1]));
+            if (nu == 3) v = v + (tc_pair(u1[j], u1[j + 1]) + tc_pair(u2[j], u2[j + 1]));
+            else v = v + tc_pair(u1[j], u1[j + 1]);
           }
-          const uint64_t old = tc_pair(st[q * 16 + j], st[q * 16 + j + 1]);
-          const float2 now = tc_unpair(tc_fma2(dec_hi, old, tc_fma2(dec_lo, old, v)));
+          const TcPair old = tc_pair(st[q * 16 + j], st[q * 16 + j + 1]);
+          const float2 now = fma2(dec_hi, old, fma2(dec_lo, old, v)).get();
           st[q * 16 + j] = now.x;
           st[q * 16 + j + 1] = now.y;
         }
@@ -647,29 +618,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
           }
         }
         unsigned char* const zw = tc_smem + L.zw + row * 128;
-        const uint64_t wt2 = tc_pair(wt, wt);
+        const TcPair wt2(wt, wt);
 #pragma unroll 1
         for (int q = 4 * part; q < 4 * part + 4; ++q) {
           const int at = (q ^ (row & 7)) << 4;
           const uint4 zv = *reinterpret_cast<const uint4*>(tc_smem + zoff + at);
           const uint32_t in[4] = {zv.x, zv.y, zv.z, zv.w};
           uint32_t t[4];
-          uint64_t v[4];
+          TcPair v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = tc_mul2(tc_widen(in[e]), wt2);
+            v[e] = tc_widen(in[e]) * wt2;
             t[e] = tc_pack(v[e]);
           }
           *reinterpret_cast<uint4*>(zw + at) = make_uint4(t[0], t[1], t[2], t[3]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = tc_sub2(v[e], tc_widen(t[e]));
+            v[e] = v[e] - tc_widen(t[e]);
             t[e] = tc_pack(v[e]);
           }
           *reinterpret_cast<uint4*>(zw + kTcPanel + at) = make_uint4(t[0], t[1], t[2], t[3]);
           if (nu == 3) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = tc_pack(tc_sub2(v[e], tc_widen(t[e])));
+            for (int e = 0; e < 4; ++e) t[e] = tc_pack(v[e] - tc_widen(t[e]));
             *reinterpret_cast<uint4*>(zw + 2 * kTcPanel + at) = make_uint4(t[0], t[1], t[2], t[3]);
           }
         }
@@ -689,9 +660,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
             uint32_t v1[4], v2[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint64_t r = tc_sub2(tc_pair(st[q * 8 + 2 * e], st[q * 8 + 2 * e + 1]), tc_widen(v[e]));
+              const TcPair r = tc_pair(st[q * 8 + 2 * e], st[q * 8 + 2 * e + 1]) - tc_widen(v[e]);
               v1[e] = tc_pack(r);
-              v2[e] = tc_pack(tc_sub2(r, tc_widen(v1[e])));
+              v2[e] = tc_pack(r - tc_widen(v1[e]));
             }
             *reinterpret_cast<uint4*>(sp + kTcPanel) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
             *reinterpret_cast<uint4*>(sp + 2 * kTcPanel) = make_uint4(v2[0], v2[1], v2[2], v2[3]);

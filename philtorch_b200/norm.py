@@ -19,13 +19,20 @@ MAX_WIDTH = 16384
 _CODES = {torch.float32: _lib.PTB_F32, torch.float64: _lib.PTB_F64, torch.float16: _lib.PTB_F16,
           torch.bfloat16: _lib.PTB_BF16}
 
-_LIB.define("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, int groups) -> (Tensor, Tensor, Tensor)",
+_LIB.define("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, int groups) -> (Tensor, Tensor)",
             tags=_TAGS)
-_LIB.define("layer_norm_bwd(Tensor x, Tensor? weight, Tensor? bias, Tensor mean, Tensor rstd, Tensor grad_y, int groups, "
+_LIB.define("layer_norm_bwd(Tensor x, Tensor? weight, Tensor? bias, Tensor stats, Tensor grad_y, int groups, "
             "bool need_x, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)", tags=_TAGS)
 
 
 def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int) -> None:
+    # the common case in one expression: the explanations below cost more host time than the launch
+    if x.dim() >= 1 and 1 <= groups <= 65535:
+        C, dt = x.shape[-1], x.dtype
+        if (C and C % groups == 0 and C // groups <= MAX_WIDTH
+                and (weight is None or (weight.shape == (C,) and weight.dtype == dt))
+                and (bias is None or (bias.shape == (C,) and bias.dtype == dt))):
+            return
     torch._check(x.dim() >= 1, lambda: "x must have at least one axis")
     C = x.shape[-1]
     torch._check(1 <= groups <= 65535 and C % groups == 0 and C > 0,
@@ -50,13 +57,18 @@ def _code(t: Tensor) -> int:
 
 def _as_rows(t: Tensor) -> Tensor:
     """(rows, channels) with dense channels; a view where the strides allow it."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _wide(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> int:
+def _wide(weight: Optional[Tensor], bias: Optional[Tensor]) -> int:
     p = weight if weight is not None else bias
     return int(p is not None and p.dtype in (torch.float32, torch.float64))
+
+
+def _stats_dtype(x: Tensor) -> torch.dtype:
+    return torch.float64 if x.dtype == torch.float64 else torch.float32
 
 
 def _layer_norm(x, weight, bias, eps, groups):
@@ -66,15 +78,19 @@ def _layer_norm(x, weight, bias, eps, groups):
     R, C = rows.shape
     w, b = (None if p is None else p.contiguous() for p in (weight, bias))
     y = x.new_empty(x.shape)
-    stats = torch.empty((2, R, groups), dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=x.device)
+    stats = x.new_empty((2, R, groups), dtype=_stats_dtype(x))
     if R:
+        at = stats.data_ptr()
         _lib.launch(lib.ptb_layer_norm_fwd, dev, _code(x), R, groups, C // groups, ptr(rows), rows.stride(0), ptr(w), ptr(b),
-                    _wide(x, weight, bias), eps, ptr(y), ptr(stats), stats.data_ptr() + stats.stride(0) * stats.element_size())
-    return y, stats[0], stats[1]
+                    _wide(weight, bias), eps, ptr(y), at, at + R * groups * stats.element_size())
+    return y, stats
 
 
-def _layer_norm_bwd(x, weight, bias, mean, rstd, grad_y, groups, need_x, need_weight, need_bias):
-    dev = _lib.require_cuda(x, weight, bias, mean, rstd, grad_y)
+_ws_bytes: dict = {}
+
+
+def _layer_norm_bwd(x, weight, bias, stats, grad_y, groups, need_x, need_weight, need_bias):
+    dev = _lib.require_cuda(x, weight, bias, stats, grad_y)
     rows, gy = _as_rows(x), _as_rows(grad_y)
     R, C = rows.shape
     w = None if weight is None else weight.contiguous()
@@ -82,10 +98,17 @@ def _layer_norm_bwd(x, weight, bias, mean, rstd, grad_y, groups, need_x, need_we
     gw = weight.new_empty((C,)) if need_weight else x.new_empty(0)
     gb = bias.new_empty((C,)) if need_bias else x.new_empty(0)
     if R:
-        code, width = _code(x), C // groups
-        ws = lib.ptb_layer_norm_bwd_workspace_bytes(code, R, groups, width) if need_weight or need_bias else 0
+        code, width, ws = _code(x), C // groups, 0
+        if need_weight or need_bias:
+            key = (code, R, groups, width)
+            ws = _ws_bytes.get(key)
+            if ws is None:
+                if len(_ws_bytes) > 4096:   # a server sees many sizes
+                    _ws_bytes.clear()
+                ws = _ws_bytes[key] = lib.ptb_layer_norm_bwd_workspace_bytes(code, R, groups, width)
+        at = stats.data_ptr()
         _lib.call(lib.ptb_layer_norm_bwd, dev, R, C, code, R, groups, width, ptr(rows), rows.stride(0), ptr(w),
-                  _wide(x, weight, bias), ptr(mean.contiguous()), ptr(rstd.contiguous()), ptr(gy), gy.stride(0),
+                  _wide(weight, bias), at, at + R * groups * stats.element_size(), ptr(gy), gy.stride(0),
                   ptr(gx) if need_x else None, ptr(gw) if need_weight else None, ptr(gb) if need_bias else None, ws_bytes=ws)
     else:
         gw.zero_()
@@ -100,13 +123,11 @@ _LIB.impl("layer_norm_bwd", _layer_norm_bwd, "CUDA")
 @torch.library.register_fake("philtorch_b200::layer_norm")
 def _(x, weight, bias, eps, groups):
     _check(x, weight, bias, groups)
-    rows = x.numel() // x.shape[-1]
-    stats = torch.float64 if x.dtype == torch.float64 else torch.float32
-    return x.new_empty(x.shape), x.new_empty((rows, groups), dtype=stats), x.new_empty((rows, groups), dtype=stats)
+    return x.new_empty(x.shape), x.new_empty((2, x.numel() // x.shape[-1], groups), dtype=_stats_dtype(x))
 
 
 @torch.library.register_fake("philtorch_b200::layer_norm_bwd")
-def _(x, weight, bias, mean, rstd, grad_y, groups, need_x, need_weight, need_bias):
+def _(x, weight, bias, stats, grad_y, groups, need_x, need_weight, need_bias):
     C = x.shape[-1]
     return (x.new_empty(x.shape if need_x else (0,)), weight.new_empty((C,)) if need_weight else x.new_empty(0),
             bias.new_empty((C,)) if need_bias else x.new_empty(0))
@@ -115,23 +136,37 @@ def _(x, weight, bias, mean, rstd, grad_y, groups, need_x, need_weight, need_bia
 _ops = torch.ops.philtorch_b200
 
 
+def _forward(x, weight, bias, eps, groups):
+    if x.device.type == "cpu":
+        _lib.require_cuda(x)
+    return (_layer_norm if _lib.eager(x) else _ops.layer_norm)(x, weight, bias, eps, groups)
+
+
+def _backward(ctx: Any, grad_y: Tensor):
+    x, weight, bias, stats = ctx.saved_tensors
+    need = ctx.needs_input_grad[:3]
+    run = _layer_norm_bwd if _lib.eager(x) else _ops.layer_norm_bwd
+    gx, gw, gb = run(x, weight, bias, stats, grad_y, ctx.groups, *need)
+    return gx if need[0] else None, gw if need[1] else None, gb if need[2] else None, None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class LayerNorm(Function):
     """(x, weight or None, bias or None, eps, groups) -> y; first derivatives."""
 
     @staticmethod
     def forward(ctx: Any, x, weight, bias, eps: float, groups: int):
-        y, mean, rstd = _ops.layer_norm(x, weight, bias, eps, groups)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = _forward(x, weight, bias, eps, groups)
+        ctx.save_for_backward(x, weight, bias, stats)
         ctx.groups = groups
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad_y: Tensor):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad[:3]
-        grads = _ops.layer_norm_bwd(x, weight, bias, mean, rstd, grad_y, ctx.groups, *need)
-        return (*(g if n else None for g, n in zip(grads, need)), None, None)
+        # (the guard against second derivatives is only needed, and only paid, where a graph is being recorded)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_y)
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
@@ -149,7 +184,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
         Tensor of x's shape and type.  Differentiable once in x, weight and bias; their gradients are sums
         in a fixed order (bit-reproducible).
     """
-    _lib.require_cuda(x, weight, bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return LayerNorm.apply(x, weight, bias, float(eps), int(groups))
-    return _ops.layer_norm(x, weight, bias, float(eps), int(groups))[0]
+    return _forward(x, weight, bias, float(eps), int(groups))[0]

@@ -24,8 +24,8 @@ def test_shapes_on_meta_tensors():
     grads = ops.linear_attention_bwd(q, q, v, g, None, None, 1.0, v, None, True, False, True, True, False)
     assert [tuple(t.shape) for t in grads] == [(2, 9, 3, 16), (0,), (2, 9, 3, 8), (3,), (0,)]
     assert ops.linear_attention_step(q[:, 0], q[:, 0], v[:, 0], g, meta(2, 3, 16, 8), 1.0).shape == (2, 3, 8)
-    y, mean, rstd = ops.layer_norm(meta(2, 5, 24), None, None, 1e-5, 3)
-    assert y.shape == (2, 5, 24) and mean.shape == rstd.shape == (10, 3)
+    y, stats = ops.layer_norm(meta(2, 5, 24), None, None, 1e-5, 3)
+    assert y.shape == (2, 5, 24) and stats.shape == (2, 10, 3)
     for bad in (lambda: ops.linear_attention(q, q, v, meta(4), None, None, 1.0, True),
                 lambda: ops.linear_attention(q, q, v.float(), g, None, None, 1.0, True),
                 lambda: ops.linear_attention(meta(2, 9, 3, 129), meta(2, 9, 3, 129), meta(2, 9, 3, 8), g, None, None, 1.0, True),
@@ -62,11 +62,12 @@ def test_c_entry_points_refuse():
     assert fwd(dtype=2) == 1 and fwd(dtype=9) == 1          # no complex numbers
     assert fwd(B=-1) == 1 and fwd(Dk=0) == 1 and fwd(Dk=129) == 1 and fwd(Dv=129) == 1
     assert fwd(q=None) == 1
-    assert fwd() == 2                                       # no workspace
-    assert fwd(ws=256, wsb=0) == 2 and fwd(ws=257, wsb=1 << 30) == 2
+    # a row long enough to be cut needs a workspace, and it has to be aligned
+    assert fwd(T=1 << 20) == 2 and fwd(T=1 << 20, ws=256, wsb=64) == 2 and fwd(T=1 << 20, ws=257, wsb=1 << 30) == 2
     assert fwd(B=0) == 0 and fwd(H=0) == 0
     assert fwd(B=1 << 20, H=1 << 20) == 4
-    assert lib.ptb_linear_attention_workspace_bytes(0, 1, 4, 1, 8, 8, 0, 0) > 0
+    assert lib.ptb_linear_attention_workspace_bytes(0, 1, 4, 1, 8, 8, 0, 0) == 0
+    assert lib.ptb_linear_attention_workspace_bytes(0, 1, 1 << 20, 1, 8, 8, 0, 0) > 0
     assert lib.ptb_linear_attention_workspace_bytes(2, 1, 4, 1, 8, 8, 0, 0) == 0
     # the gradient of the decays keeps the states at the chunks' ends
     plain = lib.ptb_linear_attention_workspace_bytes(5, 1, 4096, 4, 128, 128, 1, 0)
