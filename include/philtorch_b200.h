@@ -501,7 +501,7 @@ int ptb_modal_bank_bwd(int dtype, int64_t rows, int64_t M, int64_t N, const void
  * axis dense; *_strides: three element strides (batch, time, head), zero where an axis is shared.  log_decay likewise
  * (batch and time stride zero: one decay per head); -inf is a decay of zero.  lengths: optional (B,), clamped to
  * 0..T: tokens from lengths[b] on are not read, leave the state alone and give zeros.  init, fin: optional dense
- * (B,H,Dk,Dv), the state before the first and after the last token.  o: dense (B,T,H,Dv).
+ * (B,H,Dk,Dv), the state before the first and after the last token.  o: dense (B,T,H,Dv), float32 when o_wide.
  * workspace: ptb_linear_attention_workspace_bytes(..., backward, decay_grad) bytes, 256-byte aligned, private to the
  * call until it completes; none (NULL) where that is 0.  status: as above (waits inside a CTA are bounded). */
 int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
@@ -509,7 +509,7 @@ int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, in
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const int32_t* lengths, const void* init, double scale, void* o, void* fin,
+                             const int32_t* lengths, const void* init, double scale, void* o, int o_wide, void* fin,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream);
 /* Adjoint: the gradients of q, k, v (dense, shaped like them), of the log decays ((B,T,H) when
  * grad_log_decay_per_token, else (H)) and of the initial state, each optional.  grad_fin: optional gradient of fin.
@@ -529,14 +529,15 @@ int ptb_linear_attention_step(int dtype, int64_t B, int64_t H, int64_t Dk, int64
                               double scale, void* state, const int64_t* state_strides, void* o, ptb_stream_t stream);
 
 /* ---- layer norm over groups of channels --------------------------------------------------------
- * x: rows of groups * width channels (dense), x_stride elements apart; y dense.  weight, bias: optional
- * (groups * width), of the storage type, or float32 / float64 when params_wide.  mean, rstd: (rows, groups) in float32
+ * x: rows of groups * width channels (dense), x_stride elements apart; y dense, of y_dtype: x's, or PTB_F16 / PTB_BF16
+ * beside float32 x.  weight, bias: optional
+ * (groups * width), of y's type, or float32 / float64 when params_wide.  mean, rstd: (rows, groups) in float32
  * (float64 beside PTB_F64), written by the forward call (both optional there) and read by the adjoint.
  * 1 <= width <= 16384, groups <= 65535.  The parameter gradients have the parameters' type. */
 int64_t ptb_layer_norm_bwd_workspace_bytes(int dtype, int64_t rows, int64_t groups, int64_t width);
 int ptb_layer_norm_fwd(int dtype, int64_t rows, int64_t groups, int64_t width, const void* x, int64_t x_stride,
-                       const void* weight, const void* bias, int params_wide, double eps, void* y, void* mean,
-                       void* rstd, ptb_stream_t stream);
+                       const void* weight, const void* bias, int params_wide, double eps, int y_dtype, void* y,
+                       void* mean, void* rstd, ptb_stream_t stream);
 int ptb_layer_norm_bwd(int dtype, int64_t rows, int64_t groups, int64_t width, const void* x, int64_t x_stride,
                        const void* weight, int params_wide, const void* mean, const void* rstd, const void* grad_y,
                        int64_t grad_y_stride, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,

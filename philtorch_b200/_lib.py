@@ -160,7 +160,7 @@ _strides = ctypes.POINTER(_i64)
 _la_in = [_i32] + [_i64] * 5 + [_vp, _strides] * 4 + [_vp, _vp, ctypes.c_double]
 lib.ptb_linear_attention_workspace_bytes.argtypes = [_i32] + [_i64] * 5 + [_i32, _i32]
 lib.ptb_linear_attention_workspace_bytes.restype = _i64
-lib.ptb_linear_attention_fwd.argtypes = _la_in + [_vp, _vp] + _tail
+lib.ptb_linear_attention_fwd.argtypes = _la_in + [_vp, _i32, _vp] + _tail
 lib.ptb_linear_attention_fwd.restype = _i32
 lib.ptb_linear_attention_bwd.argtypes = _la_in + [_vp, _strides] + [_vp] * 5 + [_i32, _vp] + _tail
 lib.ptb_linear_attention_bwd.restype = _i32
@@ -169,7 +169,7 @@ lib.ptb_linear_attention_step.argtypes = ([_i32] + [_i64] * 4 + [_vp, _strides] 
 lib.ptb_linear_attention_step.restype = _i32
 lib.ptb_layer_norm_bwd_workspace_bytes.argtypes = [_i32] + [_i64] * 3
 lib.ptb_layer_norm_bwd_workspace_bytes.restype = _i64
-lib.ptb_layer_norm_fwd.argtypes = [_i32] + [_i64] * 3 + [_vp, _i64, _vp, _vp, _i32, ctypes.c_double] + [_vp] * 3 + [_vp]
+lib.ptb_layer_norm_fwd.argtypes = [_i32] + [_i64] * 3 + [_vp, _i64, _vp, _vp, _i32, ctypes.c_double, _i32] + [_vp] * 3 + [_vp]
 lib.ptb_layer_norm_fwd.restype = _i32
 lib.ptb_layer_norm_bwd.argtypes = ([_i32] + [_i64] * 3 + [_vp, _i64, _vp, _i32] + [_vp] * 3 + [_i64] + [_vp] * 3 + _tail)
 lib.ptb_layer_norm_bwd.restype = _i32

@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import lib, ptr
-from .norm import layer_norm
+from .norm import layer_norm, layer_norm_of_sums
 from .ops import _LIB, _TAGS
 
 __all__ = ["LinearAttention", "MAX_HEAD_DIM"]
@@ -120,7 +120,7 @@ def _int_lengths(lengths: Optional[Tensor], T: int) -> Optional[Tensor]:
 
 # ------------------------------------------------------------------------------------------------ ops
 _LIB.define("linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? init, Tensor? lengths, "
-            "float scale, bool want_state) -> (Tensor, Tensor)", tags=_TAGS)
+            "float scale, bool want_state, bool wide=False) -> (Tensor, Tensor)", tags=_TAGS)
 _LIB.define("linear_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? init, Tensor? lengths, "
             "float scale, Tensor? grad_o, Tensor? grad_state, bool need_q, bool need_k, bool need_v, "
             "bool need_decay, bool need_init) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", tags=_TAGS)
@@ -128,7 +128,7 @@ _LIB.define("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_deca
             "-> Tensor", tags=_TAGS)
 
 
-def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state):
+def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state, wide=False):
     _check(q, k, v, log_decay, init, lengths)
     dev = _lib.require_cuda(q, k, v, log_decay, init, lengths)
     code = _code(q)
@@ -137,12 +137,12 @@ def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state):
     q, k, v = _rows(q), _rows(k), _rows(v)
     init = None if init is None else init.contiguous()
     lengths = _int_lengths(lengths, T)
-    o = v.new_empty((B, T, H, Dv))
+    o = (log_decay if wide else v).new_empty((B, T, H, Dv))   # wide: in the sums' type, for a normalisation that follows
     state = log_decay.new_empty((B, H, Dk, Dv) if want_state else (0,))
     if B and H and (T or want_state):
         _lib.call(lib.ptb_linear_attention_fwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides3(q), ptr(k), _strides3(k),
                   ptr(v), _strides3(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(o),
-                  ptr(state) if want_state else None, ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 0, 0))
+                  int(o.dtype != v.dtype), ptr(state) if want_state else None, ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 0, 0))
     return o, state
 
 
@@ -228,10 +228,10 @@ _LIB.impl("linear_attention_step", _linear_attention_step, "CUDA")
 
 
 @torch.library.register_fake("philtorch_b200::linear_attention")
-def _(q, k, v, log_decay, init, lengths, scale, want_state):
+def _(q, k, v, log_decay, init, lengths, scale, want_state, wide=False):
     _check(q, k, v, log_decay, init, lengths)
     B, T, H, Dk = q.shape
-    return v.new_empty((B, T, H, v.shape[3])), log_decay.new_empty((B, H, Dk, v.shape[3]) if want_state else (0,))
+    return (log_decay if wide else v).new_empty((B, T, H, v.shape[3])), log_decay.new_empty((B, H, Dk, v.shape[3]) if want_state else (0,))
 
 
 @torch.library.register_fake("philtorch_b200::linear_attention_bwd")
@@ -252,11 +252,11 @@ _ops = torch.ops.philtorch_b200
 
 
 # ------------------------------------------------------------------------------------------------ autograd
-def _forward(q, k, v, log_decay, init, lengths, scale, want_state):
+def _forward(q, k, v, log_decay, init, lengths, scale, want_state, wide=False):
     if q.device.type == "cpu":
         _lib.require_cuda(q)
     run = _linear_attention if _lib.eager(q) else _ops.linear_attention
-    return run(q, k, v, log_decay, init, lengths, scale, want_state)
+    return run(q, k, v, log_decay, init, lengths, scale, want_state, wide)
 
 
 def _backward(ctx: Any, grad_o: Optional[Tensor], grad_state: Optional[Tensor]):
@@ -292,13 +292,18 @@ class LinearAttention(Function):
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_o, grad_state)
 
 
-def _normalised(o: Tensor, eps: Optional[float], weight: Optional[Tensor], bias: Optional[Tensor]) -> Tensor:
+def _normalised(o: Tensor, dtype: torch.dtype, eps: Optional[float], weight: Optional[Tensor], bias: Optional[Tensor]) -> Tensor:
     if eps is None:
-        if weight is not None or bias is not None:
-            raise ValueError("norm_weight and norm_bias need norm_eps")
-        return o
+        raise ValueError("norm_weight and norm_bias need norm_eps")
     H, Dv = o.shape[-2:]
-    return layer_norm(o.flatten(-2), weight, bias, eps=eps, groups=H).unflatten(-1, (H, Dv))
+    rows = o.flatten(-2)
+    if o.dtype == dtype:
+        return layer_norm(rows, weight, bias, eps=eps, groups=H).unflatten(-1, (H, Dv))
+    return layer_norm_of_sums(rows, weight, bias, float(eps), H, dtype).unflatten(-1, (H, Dv))
+
+
+def _norm_differentiable(*params: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(p is not None and p.requires_grad for p in params)
 
 
 def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tensor], scale: float,
@@ -308,10 +313,11 @@ def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tens
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or (zi is not None and zi.requires_grad)):
         o, state = LinearAttention.apply(q, k, v, log_decay, zi, lengths, float(scale), want)
-    else:
-        o, state = _forward(q, k, v, log_decay, zi, lengths, float(scale), want)
+    else:   # (without gradients the normalisation reads the sums before they are rounded to q's type)
+        wide = norm_eps is not None and not _norm_differentiable(norm_weight, norm_bias)
+        o, state = _forward(q, k, v, log_decay, zi, lengths, float(scale), want, wide)
     if norm_eps is not None or norm_weight is not None or norm_bias is not None:
-        o = _normalised(o, norm_eps, norm_weight, norm_bias)
+        o = _normalised(o, q.dtype, norm_eps, norm_weight, norm_bias)
     return (o, state) if want else o
 
 
@@ -326,5 +332,5 @@ def attend_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tenso
     run = _linear_attention_step if _lib.eager(q) else _ops.linear_attention_step
     o = run(q, k, v, log_decay, state, float(scale))
     if norm_eps is not None or norm_weight is not None or norm_bias is not None:
-        o = _normalised(o, norm_eps, norm_weight, norm_bias)
+        o = _normalised(o, q.dtype, norm_eps, norm_weight, norm_bias)
     return o

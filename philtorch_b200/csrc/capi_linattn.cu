@@ -312,7 +312,7 @@ static void la_strides(int64_t (&d)[3], const int64_t* s) { for (int i = 0; i < 
 template <class T, class S>
 static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs,
                   const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
-                  const int64_t* gs, const int32_t* lengths, const void* init, double scale, void* o, void* fin,
+                  const int64_t* gs, const int32_t* lengths, const void* init, double scale, void* o, int o_wide, void* fin,
                   void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
   LaArgs<S> a = {};
   LaPass<S>& p = a.p[0];
@@ -323,6 +323,7 @@ static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
   p.fin = static_cast<S*>(fin);
   p.M = (int)Dk; p.N = (int)Dv;
   p.po = (S)scale; p.pz = (S)1;
+  p.wide = o_wide;
   a.g = static_cast<const S*>(g);
   la_strides(a.gs, gs);
   a.lengths = lengths;
@@ -473,13 +474,13 @@ int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, in
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const int32_t* lengths, const void* init, double scale, void* o, void* fin,
+                             const int32_t* lengths, const void* init, double scale, void* o, int o_wide, void* fin,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
   if (int rc = la_check(dtype, B, T, H, Dk, Dv)) return rc;
   if (B == 0 || H == 0) return PTB_OK;
   if ((T > 0 && (!q || !k || !v || !o || !log_decay)) || !q_strides || !k_strides || !v_strides || !log_decay_strides) return PTB_ERR_ARG;
   PTB_LA_TYPES((la_fwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
-                               lengths, init, scale, o, fin, workspace, workspace_bytes, status, (cudaStream_t)stream)))
+                               lengths, init, scale, o, o_wide, fin, workspace, workspace_bytes, status, (cudaStream_t)stream)))
 }
 
 int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,

@@ -21,7 +21,8 @@ static int64_t ln_row_blocks(int64_t rows, int groups, int L, int64_t per_sm) {
 }
 static int64_t ln_bwd_blocks(int64_t rows, int groups, int L) { return ln_row_blocks(rows, groups, L, L > 256 ? 1 : 2); }
 
-template <class T, class S, int V, int L, int NV>
+// T: x's type, TO: y's
+template <class T, class TO, class S, int V, int L, int NV>
 static int ln_launch(const LnArgs<S>& a, bool bwd, int64_t blocks, cudaStream_t st) {
   constexpr int NT = ln_threads(L), SLOTS = NT / L;
   constexpr int kPipe = ln_pipe_bytes<T, S, V, L, NV>(1), kPipeBwd = ln_pipe_bytes<T, S, V, L, NV>(2);
@@ -32,16 +33,17 @@ static int ln_launch(const LnArgs<S>& a, bool bwd, int64_t blocks, cudaStream_t 
   {
     std::lock_guard<std::mutex> lock(init_mutex());
     if (!ready[dev]) {
-      PTB_CUDA(cudaFuncSetAttribute(ln_fwd_kernel<T, S, V, L, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPipe));
-      PTB_CUDA(cudaFuncSetAttribute(ln_bwd_kernel<T, S, V, L, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    std::max(kPipeBwd, 48 * 1024)));
+      PTB_CUDA(cudaFuncSetAttribute(ln_fwd_kernel<T, TO, S, V, L, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPipe));
+      if constexpr (std::is_same<T, TO>::value)
+        PTB_CUDA(cudaFuncSetAttribute(ln_bwd_kernel<T, S, V, L, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      std::max(kPipeBwd, 48 * 1024)));
       ready[dev] = true;
     }
   }
   if (!bwd) {
     const int64_t grid = ln_row_blocks(a.rows, a.groups, L, 8);
-    ln_fwd_kernel<T, S, V, L, NV><<<dim3((unsigned)grid, a.groups), NT, kPipe, st>>>(a);
-  } else {
+    ln_fwd_kernel<T, TO, S, V, L, NV><<<dim3((unsigned)grid, a.groups), NT, kPipe, st>>>(a);
+  } else if constexpr (std::is_same<T, TO>::value) {
     const int join = SLOTS > 1 ? SLOTS * a.width * (int)sizeof(S) : 0;   // at most 256 * V * NV scalars = 32 KB
     ln_bwd_kernel<T, S, V, L, NV><<<dim3((unsigned)blocks, a.groups), NT, std::max(kPipeBwd, join), st>>>(a);
   }
@@ -49,10 +51,10 @@ static int ln_launch(const LnArgs<S>& a, bool bwd, int64_t blocks, cudaStream_t 
   return PTB_OK;
 }
 
-template <class T, class S, int V>
+template <class T, class TO, class S, int V>
 static int ln_pick(const LnArgs<S>& a, bool bwd, int64_t blocks, cudaStream_t st) {
   const int L = ln_lanes(a.width, V), nv = (a.width + L * V - 1) / (L * V);
-#define PTB_LN(L_, N_) return ln_launch<T, S, V, L_, N_>(a, bwd, blocks, st)
+#define PTB_LN(L_, N_) return ln_launch<T, TO, S, V, L_, N_>(a, bwd, blocks, st)
   if (L == 8) { if (nv <= 1) PTB_LN(8, 1); if (nv <= 2) PTB_LN(8, 2); PTB_LN(8, 4); }
   if (L == 32) { if (nv <= 2) PTB_LN(32, 2); PTB_LN(32, 4); }
   if (L == 256) { if (nv <= 2) PTB_LN(256, 2); PTB_LN(256, 4); }
@@ -71,10 +73,19 @@ static int ln_vec(const LnArgs<S>& a) {   // elements per access
   return ok ? V : 1;
 }
 
-template <class T, class S>
+template <class T, class TO, class S>
 static int ln_fwd(const LnArgs<S>& a, cudaStream_t st) {
-  if (ln_vec<T, S>(a) == 1) return ln_pick<T, S, 1>(a, false, 0, st);
-  return ln_pick<T, S, 16 / sizeof(T)>(a, false, 0, st);
+  if (ln_vec<T, S>(a) == 1) return ln_pick<T, TO, S, 1>(a, false, 0, st);
+  return ln_pick<T, TO, S, 16 / sizeof(T)>(a, false, 0, st);
+}
+
+template <class T, class S>
+static int ln_fwd_to(const LnArgs<S>& a, int y_dtype, cudaStream_t st) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (y_dtype == PTB_F16) return ln_fwd<float, __half, float>(a, st);
+    if (y_dtype == PTB_BF16) return ln_fwd<float, __nv_bfloat16, float>(a, st);
+  }
+  return ln_fwd<T, T, S>(a, st);
 }
 
 template <class T, class S>
@@ -87,7 +98,7 @@ static int ln_bwd(LnArgs<S>& a, void* gw, void* gb, void* ws, int64_t wsb, cudaS
   char* w = static_cast<char*>(ws);
   a.part_w = gw ? reinterpret_cast<S*>(w) : nullptr;
   a.part_b = gb ? reinterpret_cast<S*>(w + (gw ? one : 0)) : nullptr;
-  const int rc = V == 1 ? ln_pick<T, S, 1>(a, true, blocks, st) : ln_pick<T, S, 16 / sizeof(T)>(a, true, blocks, st);
+  const int rc = V == 1 ? ln_pick<T, T, S, 1>(a, true, blocks, st) : ln_pick<T, T, S, 16 / sizeof(T)>(a, true, blocks, st);
   if (rc != PTB_OK || !need) return rc;
   ln_param_grad_kernel<T, S><<<dim3((unsigned)((C + 31) / 32), 2), 256, 0, st>>>(a.part_w, a.part_b, (int)blocks, C, gw, gb,
                                                                                a.w_wide);
@@ -137,13 +148,14 @@ int64_t ptb_layer_norm_bwd_workspace_bytes(int dtype, int64_t rows, int64_t grou
 }
 
 int ptb_layer_norm_fwd(int dtype, int64_t rows, int64_t groups, int64_t width, const void* x, int64_t x_stride,
-                       const void* weight, const void* bias, int params_wide, double eps, void* y, void* mean,
-                       void* rstd, ptb_stream_t stream) {
+                       const void* weight, const void* bias, int params_wide, double eps, int y_dtype, void* y,
+                       void* mean, void* rstd, ptb_stream_t stream) {
   if (int rc = ln_check(dtype, rows, groups, width)) return rc;
+  if (y_dtype != dtype && !(dtype == PTB_F32 && (y_dtype == PTB_F16 || y_dtype == PTB_BF16))) return PTB_ERR_ARG;
   if (rows == 0) return PTB_OK;
   if (!x || !y) return PTB_ERR_ARG;
   PTB_LN_TYPES(LnArgs<S_> a = ln_args<S_>(rows, groups, width, x, x_stride, weight, bias, params_wide, mean, rstd);
-               a.y = y; a.eps = (S_)eps; return (ln_fwd<T_, S_>(a, (cudaStream_t)stream));)
+               a.y = y; a.eps = (S_)eps; return (ln_fwd_to<T_, S_>(a, y_dtype, (cudaStream_t)stream));)
 }
 
 int ptb_layer_norm_bwd(int dtype, int64_t rows, int64_t groups, int64_t width, const void* x, int64_t x_stride,

@@ -147,7 +147,7 @@ template <int N> __device__ __forceinline__ void ln_arrived() { asm volatile("cp
 
 // grid: (row blocks, groups).  A thread keeps its channels, so it keeps its weights and biases, and asks for the
 // next row's values while it works on this one's.
-template <class T, class S, int V, int L, int NV>
+template <class T, class TO, class S, int V, int L, int NV>
 __global__ void __launch_bounds__(ln_threads(L), ln_resident(L, NV * V)) ln_fwd_kernel(const LnArgs<S> a) {
   constexpr int NT = ln_threads(L), SLOTS = NT / L, P = kLnPairs<S, V>;
   __shared__ S sm[32];
@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(ln_threads(L), ln_resident(L, NV * V)) ln_fwd_
     S wv[V], bv[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) wv[i] = 1, bv[i] = 0;
-    if (a.w && c < a.width) ln_param<T, S, V>(wv, a.w, a.w_wide, a.w_vec, (int64_t)grp * a.width + c);
-    if (a.b && c < a.width) ln_param<T, S, V>(bv, a.b, a.w_wide, a.w_vec, (int64_t)grp * a.width + c);
+    if (a.w && c < a.width) ln_param<TO, S, V>(wv, a.w, a.w_wide, a.w_vec, (int64_t)grp * a.width + c);
+    if (a.b && c < a.width) ln_param<TO, S, V>(bv, a.b, a.w_wide, a.w_vec, (int64_t)grp * a.width + c);
     ln_pairs<S, V>(w[k], wv);
     ln_pairs<S, V>(b[k], bv);
   }
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(ln_threads(L), ln_resident(L, NV * V)) ln_fwd_
         a.mean[u] = mu;
         a.rstd[u] = r;
       }
-      T* y = static_cast<T*>(a.y) + u * a.width;
+      TO* y = static_cast<TO*>(a.y) + u * a.width;
       const Pair<S> r2(r, r);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(ln_threads(L), ln_resident(L, NV * V)) ln_fwd_
         for (int i = 0; i < P; ++i) v[k][i] = fma2(v[k][i] * r2, w[k][i], b[k][i]);
         S f[V];
         ln_scalars<S, V>(f, v[k]);
-        ln_store<T, S, V>(y + c, f);
+        ln_store<TO, S, V>(y + c, f);
       }
     }
   }

@@ -35,6 +35,7 @@ struct LaPass {
   S* dots;          // may be NULL: per token w[t].o[t] of the part inside the chunk and of the entering state,
                     //   [slice][bh][t][2]
   int M, N, state_t, reverse;
+  int wide;         // o holds float32 beside a 2-byte type (for a normalisation that follows)
   S po, pz;
 };
 
@@ -159,10 +160,11 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
     const int n = (int)max((int64_t)0, min((int64_t)C, len - t0));   // valid tokens
     if (n == 0) {            // behind the sequence: zeros come out, the state stays
       if (!STATES_ONLY && p.o) {
-        T* o = static_cast<T*>(p.o);
         for (int i = tid; i < C * nw; i += 256) {
-          const int64_t t = t0 + i / nw;
-          if (t < a.T) la_store<T, S>(o + ((b * a.T + t) * a.H + h) * N + n0 + i % nw, (S)0);
+          const int64_t t = t0 + i / nw, at = ((b * a.T + t) * a.H + h) * N + n0 + i % nw;
+          if (t >= a.T) continue;
+          if (p.wide) static_cast<S*>(p.o)[at] = (S)0;
+          else la_store<T, S>(static_cast<T*>(p.o) + at, (S)0);
         }
       }
       continue;
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
         const int64_t t = t0 + r;
         const S win = sm.win[r];
         S d0 = 0, d1 = 0;
-        T* o = static_cast<T*>(p.o) + ((b * a.T + t) * a.H + h) * N + n0;
+        const int64_t at = ((b * a.T + t) * a.H + h) * N + n0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int q = tn * 4 + j;
@@ -284,7 +286,11 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
             d0 += in * wv;
             d1 += ex * wv;
           }
-          if (p.o && t < a.T && q < nw) la_store<T, S>(o + q, r < n ? in + ex : (S)0);
+          if (p.o && t < a.T && q < nw) {
+            const S v = r < n ? in + ex : (S)0;
+            if (p.wide) static_cast<S*>(p.o)[at + q] = v;
+            else la_store<T, S>(static_cast<T*>(p.o) + at + q, v);
+          }
         }
         if (p.dots) {
 #pragma unroll

@@ -170,10 +170,11 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
     }
     if (n == 0) {      // behind the sequence: zeros come out, the state stays
       if (!STATES_ONLY && p.o) {
-        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.o);
         for (int i = tid; i < C * N; i += 128) {
-          const int64_t t = t0 + i / N;
-          if (t < a.T) o[((b * a.T + t) * a.H + h) * N + i % N] = __float2bfloat16_rn(0.f);
+          const int64_t t = t0 + i / N, at = ((b * a.T + t) * a.H + h) * N + i % N;
+          if (t >= a.T) continue;
+          if (p.wide) static_cast<float*>(p.o)[at] = 0.f;
+          else static_cast<__nv_bfloat16*>(p.o)[at] = __float2bfloat16_rn(0.f);
         }
       }
       continue;
@@ -359,20 +360,24 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
           }
       }
       if (p.o) {
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.o);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int r = 16 * i + g4 + e * 8;
             if (t0 + r >= a.T) continue;
-            __nv_bfloat16* row = dst + ((b * a.T + t0 + r) * a.H + h) * N;
+            const int64_t at = ((b * a.T + t0 + r) * a.H + h) * N;
+            __nv_bfloat16* row = static_cast<__nv_bfloat16*>(p.o) + at;
+            float* wide = static_cast<float*>(p.o) + at;
             const bool on = r < n;
 #pragma unroll
             for (int q = 0; q < NJ * 2; ++q) {
               const int col = nw + 8 * q + 2 * t4;
               const float v0 = on ? o[i][q][2 * e] * p.po : 0.f, v1 = on ? o[i][q][2 * e + 1] * p.po : 0.f;
-              if (VEC) {   // N is a multiple of 8
+              if (p.wide) {
+                if (col < N) wide[col] = v0;
+                if (col + 1 < N) wide[col + 1] = v1;
+              } else if (VEC) {   // N is a multiple of 8
                 if (col < N) *reinterpret_cast<uint32_t*>(row + col) = la_pack(v0, v1);
               } else {
                 if (col < N) row[col] = __float2bfloat16_rn(v0);

@@ -248,13 +248,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   TcFactors* const fac = reinterpret_cast<TcFactors*>(tc_smem + L.misc + C * 20);   // [2]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(tc_smem + L.misc + C * 20 + 128);
   uint64_t *const xy_full = bars, *const xy_empty = bars + 2, *const zw_full = bars + 4, *const zw_empty = bars + 6;
-  uint64_t *const b_sc = bars + 8, *const b_p = bars + 9, *const b_o = bars + 10, *const b_ofree = bars + 11;
+  uint64_t *const b_sc = bars + 8, *const b_p = bars + 9, *const b_o = bars + 10, *const b_ofree = bars + 20;   // [2]
   uint64_t *const b_zw = bars + 12, *const b_u = bars + 13, *const b_s = bars + 14, *const b_oi = bars + 15;
   uint64_t *const lg_full = bars + 16, *const lg_empty = bars + 18;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   volatile uint32_t* const gave_up = tmem_slot + 1;
-  // columns of tensor memory; without dots the terms of U stand side by side, with them they add up in one
-  constexpr uint32_t kSC = 0, kP = 128, kO = 192, kOI = 256, kU = 320, kSC2 = 384;
+  // columns of tensor memory.  Without dots O and OI are double: a chunk's rows go out while the next one's weights are
+  // formed; with dots the second scores take that place
+  constexpr int kLag = DOTS ? 0 : 1;
+  constexpr uint32_t kSC = 0, kP = 128, kO = 192, kOI = DOTS ? 256 : 320, kU = DOTS ? 320 : 448, kSC2 = 384;
 
   if (base & 1023) {   // the swizzled tiles need it; dynamic shared memory starts that way without static arrays
     if (tid == 0 && k.status) atomicOr(k.status, kErrPipelineWait);
@@ -274,6 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     mbar_init(b_p, 8);   // one arrival a warp
     mbar_init(b_o, 1);
     mbar_init(b_ofree, 8);
+    mbar_init(b_ofree + 1, 8);
     mbar_init(b_zw, 8);
     mbar_init(b_u, 1);
     mbar_init(b_s, 8);
@@ -327,52 +330,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     {   // products: the warp stays together (operands in uniform registers), one thread issues
       const bool one = tc_elect();
       constexpr uint32_t kScD = tc_idesc(128, 128, false, false), kOD = tc_idesc(128, 64, false, true),
-                         kUD = tc_idesc(128, 64, true, true), kUD2 = tc_idesc(128, 128, true, true),
-                         kUD3 = tc_idesc(128, 192, true, true);
+                         kUD = tc_idesc(128, 64, true, true);
       const uint32_t Zw = tc_desc(base + L.zw), S = tc_desc(base + L.s);
+      auto scores = [&](int i) {
+        const int s = i % sxy, sz = i & 1;
+        const uint32_t X = tc_desc(base + s * 4 * kTcPanel), Y = X + (2 * kTcPanel >> 4);
+        wait_warp(xy_full + s, (i / sxy) & 1);
+        tc_after();
+        if (one) tc_products<kKMajor, kKMajor, 8>(tm + kSC, X, Y, kScD, true);
+        if (DOTS) {
+          const uint32_t Z = tc_desc(base + L.z + sz * 2 * kTcPanel);
+          wait_warp(zw_full + sz, (i / 2) & 1);
+          tc_after();
+          if (one) tc_products<kKMajor, kKMajor, 4>(tm + kSC2, Z + (kTcPanel >> 4), Z, kScD, true);
+        }
+        if (one) tc_commit(b_sc);
+      };
+      if (!STATES_ONLY && count > 0) scores(0);
 #pragma unroll 1
       for (int i = 0; i < count; ++i) {
         const int s = i % sxy, sz = i & 1;
         const uint32_t X = tc_desc(base + s * 4 * kTcPanel), Y = X + (2 * kTcPanel >> 4),
-                       Z = tc_desc(base + L.z + sz * (DOTS ? 2 : 1) * kTcPanel);
-        wait_warp(xy_full + s, (i / sxy) & 1);
-        tc_after();
-        if (!STATES_ONLY) {
-          if (one) tc_products<kKMajor, kKMajor, 8>(tm + kSC, X, Y, kScD, true);
-          if (DOTS) {
-            wait_warp(zw_full + sz, (i / 2) & 1);
-            tc_after();
-            if (one) tc_products<kKMajor, kKMajor, 4>(tm + kSC2, Z + (kTcPanel >> 4), Z, kScD, true);
-          }
-          if (one) tc_commit(b_sc);
-        }
+                       Z = tc_desc(base + L.z + sz * (DOTS ? 2 : 1) * kTcPanel), at = kLag ? (i & 1) * 64 : 0;
+        if (STATES_ONLY) wait_warp(xy_full + s, (i / sxy) & 1);
         wait_warp(b_zw, i & 1);
         tc_after();
-        if (!DOTS) {   // one product over the terms side by side: Y is read once
-          if (one) tc_products<kMnMajor, kMnMajor, 8>(tm + kU, Y, Zw, nu == 3 ? kUD3 : kUD2, true);
-        } else {
 #pragma unroll 1
-          for (int term = nu - 1; term >= 0; --term)   // smallest first
-            if (one) tc_products<kMnMajor, kMnMajor, 8>(tm + kU, Y, Zw + term * (kTcPanel >> 4), kUD, term == nu - 1);
-        }
+        for (int term = nu - 1; term >= 0; --term)   // smallest first
+          if (one) tc_products<kMnMajor, kMnMajor, 8>(tm + kU, Y, Zw + term * (kTcPanel >> 4), kUD, term == nu - 1);
         if (one) tc_commit(b_u);
         if (!STATES_ONLY) {
           wait_warp(b_s, i & 1);
-          if (i > 0) wait_warp(b_ofree, (i - 1) & 1);
+          if (i > kLag) wait_warp(b_ofree + (kLag ? i & 1 : 0), (kLag ? (i >> 1) - 1 : i - 1) & 1);   // O and OI have been read
           tc_after();
 #pragma unroll 1
           for (int term = ns - 1; term >= 0; --term)
-            if (one) tc_products<kKMajor, kMnMajor, 8>(tm + kOI, X, S + term * (kTcPanel >> 4), kOD, term == ns - 1);
+            if (one) tc_products<kKMajor, kMnMajor, 8>(tm + kOI + at, X, S + term * (kTcPanel >> 4), kOD, term == ns - 1);
           if (one) tc_commit(b_oi);
         }
         if (one) tc_commit(xy_empty + s);
         if (!STATES_ONLY) {
           wait_warp(b_p, i & 1);
           tc_after();
-          if (one) tc_products<kTmem, kMnMajor, 8>(tm + kO, tm + kP, Z, kOD, true);
+          if (one) tc_products<kTmem, kMnMajor, 8>(tm + kO + at, tm + kP, Z, kOD, true);
           if (one) tc_commit(b_o);
         }
         if (one) tc_commit(zw_empty + sz);
+        if (!STATES_ONLY && i + 1 < count) scores(i + 1);
       }
     }
   } else if (warp == 18) {   // decays
@@ -394,7 +398,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     if constexpr (!STATES_ONLY) {   // rows
       const int quad = warp & 3, part = warp >> 2, row = 32 * quad + lane;   // two warps share 32 rows and take turns along them
       const uint32_t lanes = tm + ((uint32_t)(32 * quad) << 16);
-      __nv_bfloat16* const o = static_cast<__nv_bfloat16*>(p.o);
       {   // blocks that hold no pair stay zero
         uint32_t zero[8] = {};
         for (int q = part; q < 8; q += 2)
@@ -423,13 +426,76 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         if (part == 0) cs[row] = row_col;
       }
       const uint32_t pairs = rev ? ~0u << lane : ~0u >> (31 - lane);   // columns of the own block that count
+      // a chunk's rows to memory
+      auto out = [&](int i, float win, float pair_sum) {
+        const int64_t t0 = chunk_of(i) * C, t = t0 + row;
+        const int n = valid(chunk_of(i)), sz = i & 1;
+        const uint32_t at = lanes + (kLag ? (i & 1) * 64 : 0) + part * 32;
+        const int64_t first = ((b * a.T + t) * a.H + h) * N + n0;
+        const bool store = p.o && t < a.T;
+        TcPair ext(0.f, 0.f);
+        const TcPair win2(win, win), scale2(scale_in, scale_in);
+        uint32_t vi[2][16], vo[2][16];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          tc_ld16(vi[q], at + kOI + q * 16);
+          tc_ld16(vo[q], at + kO + q * 16);
+        }
+        tc_wait_ld();
+        tc_before();
+        arrive_warp(b_ofree + (kLag ? i & 1 : 0));   // the products may overwrite
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            TcPair r[4];
+            const int piece = 2 * (2 * part + q) + e;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = tc_pair(vi[q][e * 8 + 2 * j], vi[q][e * 8 + 2 * j + 1]) * win2;
+            if (DOTS) {
+              const uint4 wv = *reinterpret_cast<const uint4*>(tc_smem + L.z + (sz * 2 + 1) * kTcPanel + row * 128 +
+                                                              ((piece ^ (row & 7)) << 4));
+              ext = fma2(r[0], tc_widen(wv.x), fma2(r[1], tc_widen(wv.y), fma2(r[2], tc_widen(wv.z), fma2(r[3], tc_widen(wv.w), ext))));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = fma2(tc_pair(vo[q][e * 8 + 2 * j], vo[q][e * 8 + 2 * j + 1]), scale2, r[j]);
+            if (store && n0 + piece * 8 < N) {
+              if (p.wide) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  const float2 v0 = r[2 * j].get(), v1 = r[2 * j + 1].get();
+                  float4 v = make_float4(v0.x, v0.y, v1.x, v1.y);
+                  if (row >= n) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                  *reinterpret_cast<float4*>(static_cast<float*>(p.o) + first + piece * 8 + j * 4) = v;
+                }
+              } else {
+                uint4 pk = make_uint4(tc_pack(r[0]), tc_pack(r[1]), tc_pack(r[2]), tc_pack(r[3]));
+                if (row >= n) pk = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + first + piece * 8) = pk;
+              }
+            }
+          }
+        }
+        if (DOTS) {
+          arrive_warp(zw_empty + sz);
+          if (row < n) {
+            float2* d = reinterpret_cast<float2*>(p.dots + ((((int64_t)slice * 2 + part) * BH + bh) * a.T + t) * 2);
+            const float2 e = ext.get();
+            *d = make_float2(pair_sum * scale_in, e.x + e.y);
+          }
+        }
+      };
+      float last_win = 0.f;
 #pragma unroll 1
       for (int i = 0; i < count; ++i) {
-        const int64_t c = chunk_of(i), t0 = c * C;
-        const int n = valid(c), sz = i & 1;
+        const int n = valid(chunk_of(i));
         const float* const G = Gs + (i & 1) * 2 * C;
-        const TcPair own_hi = tc_pair(row_own.x, row_own.x), own_lo = tc_pair(row_own.y, row_own.y);
+        const TcPair own_hi(row_own.x, row_own.x), own_lo(row_own.y, row_own.y);
         const float mine = row_mine, win = row_win, mid1 = row_mid1, mid2 = row_mid2;
+        if (i > 0 && kLag) {   // P has been read, and every row is past its use of the last factors
+          wait_warp(b_o, (i - 1) & 1);
+          if (part == 0) cs[row] = row_col;
+        }
         asm volatile("bar.sync 1, 256;" ::: "memory");   // every row's factors are written
         wait_warp(b_sc, i & 1);
         tc_after();
@@ -484,58 +550,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         arrive_warp(b_p);
         if (lane == 0) mbar_arrive(lg_empty + (i & 1));
         if (i + 1 < count) decays(i + 1);
-        wait_warp(b_o, i & 1);
-        if (part == 0 && i + 1 < count) cs[row] = row_col;   // every row is past its use of the last ones
-        tc_after();
-        const int64_t t = t0 + row;
-        __nv_bfloat16* const dst = o ? o + ((b * a.T + t) * a.H + h) * N + n0 : nullptr;
-        TcPair ext(0.f, 0.f);
-        const TcPair win2(win, win), scale2(scale_in, scale_in);
-        uint32_t vi[2][16], vo[2][16];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          tc_ld16(vi[q], lanes + kOI + (2 * part + q) * 16);
-          tc_ld16(vo[q], lanes + kO + (2 * part + q) * 16);
-        }
-        tc_wait_ld();
-        tc_before();
-        arrive_warp(b_ofree);   // the next products may overwrite
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            TcPair r[4];
-            const int piece = 2 * (2 * part + q) + e;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = tc_pair(vi[q][e * 8 + 2 * j], vi[q][e * 8 + 2 * j + 1]) * win2;
-            if (DOTS) {
-              const uint4 wv = *reinterpret_cast<const uint4*>(tc_smem + L.z + (sz * 2 + 1) * kTcPanel + row * 128 +
-                                                              ((piece ^ (row & 7)) << 4));
-              ext = fma2(r[0], tc_widen(wv.x), fma2(r[1], tc_widen(wv.y), fma2(r[2], tc_widen(wv.z), fma2(r[3], tc_widen(wv.w), ext))));
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = fma2(tc_pair(vo[q][e * 8 + 2 * j], vo[q][e * 8 + 2 * j + 1]), scale2, r[j]);
-            uint4 pk = make_uint4(tc_pack(r[0]), tc_pack(r[1]), tc_pack(r[2]), tc_pack(r[3]));
-            if (row >= n) pk = make_uint4(0, 0, 0, 0);
-            if (dst && t < a.T && n0 + piece * 8 < N) *reinterpret_cast<uint4*>(dst + piece * 8) = pk;
-          }
-        }
-        if (DOTS) {
-          arrive_warp(zw_empty + sz);
-          if (row < n) {
-            float2* d = reinterpret_cast<float2*>(p.dots + ((((int64_t)slice * 2 + part) * BH + bh) * a.T + t) * 2);
-            const float2 e = ext.get();
-            *d = make_float2(rowsum * scale_in, e.x + e.y);
-          }
+        if (kLag) {
+          if (i > 0) out(i - 1, last_win, 0.f);   // while this chunk's products run
+          last_win = win;
+        } else {
+          wait_warp(b_o, i & 1);
+          tc_after();
+          if (part == 0 && i + 1 < count) cs[row] = row_col;   // every row is past its use of the last ones
+          out(i, win, rowsum);
         }
       }
+      if (kLag && count > 0) {
+        wait_warp(b_o, (count - 1) & 1);
+        tc_after();
+        out(count - 1, last_win, 0.f);
+      }
       // behind the sequence: zeros
-      if (o) {
+      if (p.o) {
         const int64_t first = max(c0, (len + C - 1) / C) * C, stop = min(a.T, c1 * C);
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        const int pieces = min(8, (N - n0) / 8);
+        const int pieces = min(8, (N - n0) / 8) * (p.wide ? 2 : 1), per = p.wide ? 4 : 8;
         for (int64_t t = first + tid; t < stop; t += kTcRows)
-          for (int q = 0; q < pieces; ++q) *reinterpret_cast<uint4*>(o + ((b * a.T + t) * a.H + h) * N + n0 + q * 8) = zero;
+          for (int q = 0; q < pieces; ++q) {
+            const int64_t at = ((b * a.T + t) * a.H + h) * N + n0 + q * per;
+            *reinterpret_cast<uint4*>(static_cast<char*>(p.o) + at * (16 / per)) = zero;
+          }
       }
     }
   } else {   // state: two threads hold a row m, 32 columns each
@@ -575,21 +614,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
       tc_after();
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        uint32_t u[16], u1[16], u2[16];
-        const uint32_t at = lanes + kU + part * 32 + q * 16;
-        tc_ld16(u, at);
-        if (!DOTS) {
-          tc_ld16(u1, at + 64);
-          if (nu == 3) tc_ld16(u2, at + 128);
-        }
+        uint32_t u[16];
+        tc_ld16(u, lanes + kU + part * 32 + q * 16);
         tc_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          TcPair v = tc_pair(u[j], u[j + 1]);
-          if (!DOTS) {
-            if (nu == 3) v = v + (tc_pair(u1[j], u1[j + 1]) + tc_pair(u2[j], u2[j + 1]));
-            else v = v + tc_pair(u1[j], u1[j + 1]);
-          }
+          const TcPair v = tc_pair(u[j], u[j + 1]);
           const TcPair old = tc_pair(st[q * 16 + j], st[q * 16 + j + 1]);
           const float2 now = fma2(dec_hi, old, fma2(dec_lo, old, v)).get();
           st[q * 16 + j] = now.x;

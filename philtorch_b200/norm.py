@@ -19,19 +19,20 @@ MAX_WIDTH = 16384
 _CODES = {torch.float32: _lib.PTB_F32, torch.float64: _lib.PTB_F64, torch.float16: _lib.PTB_F16,
           torch.bfloat16: _lib.PTB_BF16}
 
-_LIB.define("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, int groups) -> (Tensor, Tensor)",
+_LIB.define("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, int groups, ScalarType? out=None) "
+            "-> (Tensor, Tensor)",
             tags=_TAGS)
 _LIB.define("layer_norm_bwd(Tensor x, Tensor? weight, Tensor? bias, Tensor stats, Tensor grad_y, int groups, "
             "bool need_x, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)", tags=_TAGS)
 
 
-def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int) -> None:
+def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, out: Optional[torch.dtype] = None) -> None:
     # the common case in one expression: the explanations below cost more host time than the launch
     if x.dim() >= 1 and 1 <= groups <= 65535:
-        C, dt = x.shape[-1], x.dtype
+        C, dt = x.shape[-1], x.dtype if out is None else out
         if (C and C % groups == 0 and C // groups <= MAX_WIDTH
                 and (weight is None or (weight.shape == (C,) and weight.dtype == dt))
-                and (bias is None or (bias.shape == (C,) and bias.dtype == dt))):
+                and (bias is None or (bias.shape == (C,) and bias.dtype == dt)) and (out is None or x.dtype in (dt, torch.float32))):
             return
     torch._check(x.dim() >= 1, lambda: "x must have at least one axis")
     C = x.shape[-1]
@@ -39,10 +40,13 @@ def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: 
                  lambda: f"the last axis ({C}) must be a multiple of groups ({groups}, at most 65535)")
     torch._check(C // groups <= MAX_WIDTH, lambda: f"groups of {C // groups} channels: the kernels cover 1..{MAX_WIDTH}.")
     wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    out = x.dtype if out is None else out
+    torch._check(out == x.dtype or (x.dtype == torch.float32 and out in (torch.float16, torch.bfloat16)),
+                 lambda: f"no results in {out} of {x.dtype} tensors")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None:
             torch._check(tuple(p.shape) == (C,), lambda: f"{name} must be ({C},), got {tuple(p.shape)}")
-            torch._check(p.dtype in (x.dtype, wide), lambda: f"{name} must be {x.dtype} or {wide}, got {p.dtype}")
+            torch._check(p.dtype in (out, wide), lambda: f"{name} must be {out} or {wide}, got {p.dtype}")
     if weight is not None and bias is not None:
         torch._check(weight.dtype == bias.dtype,
                      lambda: f"weight and bias must have the same type, got {weight.dtype} and {bias.dtype}")
@@ -71,18 +75,18 @@ def _stats_dtype(x: Tensor) -> torch.dtype:
     return torch.float64 if x.dtype == torch.float64 else torch.float32
 
 
-def _layer_norm(x, weight, bias, eps, groups):
-    _check(x, weight, bias, groups)
+def _layer_norm(x, weight, bias, eps, groups, out=None):
+    _check(x, weight, bias, groups, out)
     dev = _lib.require_cuda(x, weight, bias)
     rows = _as_rows(x)
     R, C = rows.shape
     w, b = (None if p is None else p.contiguous() for p in (weight, bias))
-    y = x.new_empty(x.shape)
+    y = x.new_empty(x.shape, dtype=out)
     stats = x.new_empty((2, R, groups), dtype=_stats_dtype(x))
     if R:
         at = stats.data_ptr()
         _lib.launch(lib.ptb_layer_norm_fwd, dev, _code(x), R, groups, C // groups, ptr(rows), rows.stride(0), ptr(w), ptr(b),
-                    _wide(weight, bias), eps, ptr(y), at, at + R * groups * stats.element_size())
+                    _wide(weight, bias), eps, _code(y), ptr(y), at, at + R * groups * stats.element_size())
     return y, stats
 
 
@@ -121,9 +125,9 @@ _LIB.impl("layer_norm_bwd", _layer_norm_bwd, "CUDA")
 
 
 @torch.library.register_fake("philtorch_b200::layer_norm")
-def _(x, weight, bias, eps, groups):
-    _check(x, weight, bias, groups)
-    return x.new_empty(x.shape), x.new_empty((2, x.numel() // x.shape[-1], groups), dtype=_stats_dtype(x))
+def _(x, weight, bias, eps, groups, out=None):
+    _check(x, weight, bias, groups, out)
+    return x.new_empty(x.shape, dtype=out), x.new_empty((2, x.numel() // x.shape[-1], groups), dtype=_stats_dtype(x))
 
 
 @torch.library.register_fake("philtorch_b200::layer_norm_bwd")
@@ -167,6 +171,12 @@ class LayerNorm(Function):
     def backward(ctx: Any, grad_y: Tensor):
         # (the guard against second derivatives is only needed, and only paid, where a graph is being recorded)
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_y)
+
+
+def layer_norm_of_sums(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, groups: int,
+                       out: torch.dtype) -> Tensor:
+    """``layer_norm`` of float32 sums with results (and parameters) in a 2-byte type; no gradients."""
+    return (_layer_norm if _lib.eager(x) else _ops.layer_norm)(x, weight, bias, eps, groups, out)[0]
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,

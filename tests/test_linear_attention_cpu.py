@@ -56,7 +56,7 @@ def test_c_entry_points_refuse():
     s = I3(8, 8, 8)
 
     def fwd(dtype=0, B=1, T=4, H=1, Dk=8, Dv=8, q=p, ws=None, wsb=0):
-        return lib.ptb_linear_attention_fwd(dtype, B, T, H, Dk, Dv, q, s, p, s, p, s, p, s, None, None, 1.0, p, None, ws, wsb,
+        return lib.ptb_linear_attention_fwd(dtype, B, T, H, Dk, Dv, q, s, p, s, p, s, p, s, None, None, 1.0, p, 0, None, ws, wsb,
                                             None, None)
 
     assert fwd(dtype=2) == 1 and fwd(dtype=9) == 1          # no complex numbers
@@ -75,8 +75,9 @@ def test_c_entry_points_refuse():
     z = I2(8, 8)
     assert lib.ptb_linear_attention_step(0, 1, 1, 8, 200, p, z, p, z, p, z, p, z, 1.0, p, z, p, None) == 1
     assert lib.ptb_linear_attention_step(0, 1, 1, 8, 8, p, z, p, z, p, z, p, z, 1.0, None, z, p, None) == 1
-    assert lib.ptb_layer_norm_fwd(0, 4, 1, 16385, p, 8, None, None, 0, 1e-5, p, None, None, None) == 1
-    assert lib.ptb_layer_norm_fwd(0, 4, 0, 8, p, 8, None, None, 0, 1e-5, p, None, None, None) == 1
-    assert lib.ptb_layer_norm_fwd(0, 4, 1, 8, None, 8, None, None, 0, 1e-5, p, None, None, None) == 1
-    assert lib.ptb_layer_norm_fwd(0, 0, 1, 8, None, 8, None, None, 0, 1e-5, None, None, None, None) == 0
+    assert lib.ptb_layer_norm_fwd(0, 4, 1, 16385, p, 8, None, None, 0, 1e-5, 0, p, None, None, None) == 1
+    assert lib.ptb_layer_norm_fwd(0, 4, 0, 8, p, 8, None, None, 0, 1e-5, 0, p, None, None, None) == 1
+    assert lib.ptb_layer_norm_fwd(0, 4, 1, 8, None, 8, None, None, 0, 1e-5, 0, p, None, None, None) == 1
+    assert lib.ptb_layer_norm_fwd(5, 4, 1, 8, p, 8, None, None, 0, 1e-5, 0, p, None, None, None) == 1   # only narrowing
+    assert lib.ptb_layer_norm_fwd(0, 0, 1, 8, None, 8, None, None, 0, 1e-5, 0, None, None, None, None) == 0
     assert lib.ptb_layer_norm_bwd(0, 4, 1, 8, p, 8, None, 0, p, p, p, 8, p, p, p, None, 0, None, None) == 2
