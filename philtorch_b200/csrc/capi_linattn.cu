@@ -30,15 +30,17 @@ static void la_cut(int64_t ctas, int64_t nchunk, int64_t room, int* nseg, int* s
 
 struct LaSize { int64_t B, T, H, Dk, Dv; };
 
-// C: tokens of a chunk; slices: CTAs that share the columns of a state; mn: scalars of a stored state
+// C: tokens of a chunk; width: columns of a state that a CTA takes; mn: scalars of a stored state
 template <class S>
-static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int slices, int64_t mn, int per_sm, int slots) {
+static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int width, int64_t mn, int per_sm, int slots) {
   LaPlan l;
   l.C = C;
-  l.slices_max = slices;
+  const int64_t over_k = (z.Dk + width - 1) / width, over_v = (z.Dv + width - 1) / width;
+  l.slices_max = (int)std::max(over_k, over_v);
+  const int64_t slices = roles == 1 ? over_v : 2 * over_k + over_v;   // of o; of dq, dk and dv
   l.nchunk = (z.T + C - 1) / C;
   const int64_t BH = z.B * z.H;
-  la_cut(BH * roles * slices, l.nchunk, kLaSms * per_sm, &l.nseg, &l.seg_chunks);
+  la_cut(BH * slices, l.nchunk, kLaSms * per_sm, &l.nseg, &l.seg_chunks);
   l.seg_stride = align_up(mn, 64);
   l.bound_elems = mn;
   int64_t at = 0;
@@ -56,16 +58,16 @@ static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int sl
 template <class S>
 static LaPlan la_simt_plan(const LaSize& z, int roles, bool decay_grad) {
   using G = LaGeom<S>;
-  return la_plan<S>(z, roles, decay_grad, G::C, (int)((std::max(z.Dk, z.Dv) + G::NS - 1) / G::NS), z.Dk * z.Dv, G::PER_SM, 0);
+  return la_plan<S>(z, roles, decay_grad, G::C, G::NS, z.Dk * z.Dv, G::PER_SM, 0);
 }
 // the tensor-core kernels come for head sizes up to 64 and up to 128
 static int la_mma_width(const LaSize& z) { return std::max(z.Dk, z.Dv) <= 64 ? 64 : 128; }
 static LaPlan la_mma_plan(const LaSize& z, int roles, bool decay_grad) {
   const int64_t W = la_mma_width(z);
-  return la_plan<float>(z, roles, decay_grad, kLaMmaChunk, 1, W * W, W == 64 ? 4 : 2, 1);
+  return la_plan<float>(z, roles, decay_grad, kLaMmaChunk, kLaMaxDim, W * W, W == 64 ? 4 : 2, 1);
 }
 static LaPlan la_tc_plan(const LaSize& z, int roles, bool decay_grad) {
-  return la_plan<float>(z, roles, decay_grad, kTcChunk, 2, kTcDim * kTcDim, 1, 1);
+  return la_plan<float>(z, roles, decay_grad, kTcChunk, kTcSlice, kTcDim * kTcDim, 1, 1);
 }
 enum LaPath { kLaSimt, kLaMma, kLaTc };
 template <class S>
@@ -77,10 +79,10 @@ static LaPlan la_plan_of(LaPath path, const LaSize& z, int roles, bool decay_gra
   return la_simt_plan<S>(z, roles, decay_grad);
 }
 
-template <class T, class S, bool STATES_ONLY>
+template <class T, class S, int MD, bool STATES_ONLY>
 static int la_simt_launch(const LaArgs<S>& a, int roles, cudaStream_t st) {
   using G = LaGeom<S>;
-  constexpr int smem = sizeof(LaSimtSmem<S, G::C, G::NS>);
+  constexpr int smem = sizeof(LaSimtSmem<S, G::C, G::NS, MD>);
   static bool ready[kMaxDevices] = {};
   int dev = 0;
   PTB_CUDA(cudaGetDevice(&dev));
@@ -88,14 +90,14 @@ static int la_simt_launch(const LaArgs<S>& a, int roles, cudaStream_t st) {
   {
     std::lock_guard<std::mutex> lock(init_mutex());
     if (!ready[dev]) {
-      PTB_CUDA(cudaFuncSetAttribute(la_simt_kernel<T, S, G::C, G::NS, STATES_ONLY>,
+      PTB_CUDA(cudaFuncSetAttribute(la_simt_kernel<T, S, G::C, G::NS, MD, STATES_ONLY>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
       ready[dev] = true;
     }
   }
   const int64_t grid = a.B * a.H * (STATES_ONLY ? a.nseg - 1 : a.nseg) * ((kLaMaxDim + G::NS - 1) / G::NS);
   if (grid > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
-  la_simt_kernel<T, S, G::C, G::NS, STATES_ONLY><<<dim3((unsigned)grid, roles), 256, smem, st>>>(a);
+  la_simt_kernel<T, S, G::C, G::NS, MD, STATES_ONLY><<<dim3((unsigned)grid, roles), 256, smem, st>>>(a);
   PTB_CUDA(cudaGetLastError());
   return PTB_OK;
 }
@@ -110,15 +112,15 @@ static void la_workspace(LaArgs<S>& a, const LaPlan& l, void* ws) {
   a.seg_log = reinterpret_cast<double*>(w + l.log_off);
 }
 
-template <class T, class S>
+template <class T, class S, int MD>
 static int la_simt_run(LaArgs<S>& a, int roles, cudaStream_t st) {
   if (a.nseg > 1) {
-    if (int rc = la_simt_launch<T, S, true>(a, roles, st)) return rc;
+    if (int rc = la_simt_launch<T, S, MD, true>(a, roles, st)) return rc;
     const int64_t elems = a.B * a.H * (int64_t)a.p[0].M * a.p[0].N;
     la_join_kernel<S><<<dim3((unsigned)((elems + 255) / 256), roles), 256, 0, st>>>(a);
     PTB_CUDA(cudaGetLastError());
   }
-  return la_simt_launch<T, S, false>(a, roles, st);
+  return la_simt_launch<T, S, MD, false>(a, roles, st);
 }
 
 template <int W, bool VEC, bool STATES_ONLY>
@@ -198,10 +200,10 @@ static bool la_tc_map(LaTcMap* m, const void* base, const int64_t* st, int64_t B
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The tcgen05 kernels take head sizes above 64 (their tiles are 128 wide; up to 64 the mma.sync kernels do half the
-// work) and operands that the TMA unit can address.
+// The tcgen05 kernels take every size whose operands the TMA unit can address; the mma.sync kernels the others
+// (odd or unaligned head sizes).  B=1, H=4, D=64, T=256: 31.6 us on mma.sync, XXX us here.
 static bool la_tc_setup(LaTcArgs* k, const LaArgs<float>& a, int roles) {
-  if (std::max(a.p[0].M, a.p[0].N) <= 64 || a.T < 1 || a.T > 0x7fffffffll || !la_mma_vec(a, roles)) return false;
+  if (a.T < 1 || a.T > 0x7fffffffll || !la_mma_vec(a, roles)) return false;
   for (int r = 0; r < roles; ++r) {
     const LaPass<float>& p = a.p[r];
     if (!la_tc_map(&k->x[r], p.x, p.xs, a.B, a.T, a.H, p.M) || !la_tc_map(&k->y[r], p.y, p.ys, a.B, a.T, a.H, p.M) ||
@@ -297,7 +299,9 @@ static int la_run(LaArgs<S>& a, LaTcArgs* k, LaPath path, int roles, const LaPla
       return vec ? la_mma_run<64, true>(a, roles, dots, st) : la_mma_run<64, false>(a, roles, dots, st);
     return vec ? la_mma_run<128, true>(a, roles, dots, st) : la_mma_run<128, false>(a, roles, dots, st);
   } else {
-    return la_simt_run<T, S>(a, roles, st);
+    int most = 0;   // channels of x and y
+    for (int r = 0; r < roles; ++r) most = std::max(most, a.p[r].M);
+    return most <= 64 ? la_simt_run<T, S, 64>(a, roles, st) : la_simt_run<T, S, 128>(a, roles, st);
   }
 }
 

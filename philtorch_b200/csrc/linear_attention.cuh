@@ -94,27 +94,39 @@ __device__ __forceinline__ void la_running_logs(double* G, const S* g, int64_t t
   }
 }
 
-template <class S, int C, int NS>
+template <class S> struct LaVec4;   // four scalars, in 16-byte accesses
+template <> struct LaVec4<float> { float4 v; __device__ __forceinline__ void get(float (&d)[4]) const { d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w; } };
+template <> struct LaVec4<double> {
+  double2 a, b;
+  __device__ __forceinline__ void get(double (&d)[4]) const { d[0] = a.x; d[1] = a.y; d[2] = b.x; d[3] = b.y; }
+};
+template <class S> __device__ __forceinline__ void la_get4(S (&d)[4], const S* p) { reinterpret_cast<const LaVec4<S>*>(p)->get(d); }
+
+// MD: channels of x and y that fit (64 or 128)
+template <class S, int C, int NS, int MD>
 struct LaSimtSmem {
-  static constexpr int XLD = kLaMaxDim + 4;
+  static constexpr int XLD = MD + 4;
   S x[C][XLD], y[C][XLD];
   S z[C][NS];
-  S s[kLaMaxDim][NS];
+  S s[MD][NS];
   S p[C][C + 4];
-  S win[C], wout[C];     // weight of the entering state per row, weight with which a token joins the state
-  double G[C];
+  // two chunks' decays: weight of the entering state per row, weight with which a token joins the state, running sums
+  S win[2][C], wout[2][C];
+  double G[2][C];
 };
 
 // Float32 / float64 arithmetic on the CUDA cores, any size up to 128: the path of float32, float64 and
 // float16 tensors.  A CTA walks one (b, h, segment) in time order with a slice of NS columns of
-// the state in registers (8 x 4 per thread) and a copy in shared memory for the products that read it.
-template <class T, class S, int C, int NS, bool STATES_ONLY>
-__global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
+// the state in registers (8 x 4 per thread in float32) and a copy in shared memory for the products that read it.
+// Two CTAs an SM: one's barriers and loads lie under the other's arithmetic.
+template <class T, class S, int C, int NS, int MD, bool STATES_ONLY>
+__global__ void __launch_bounds__(256, sizeof(S) == 4 ? 2 : 1) la_simt_kernel(const LaArgs<S> a) {
   extern __shared__ __align__(16) unsigned char la_smem[];
-  using Sm = LaSimtSmem<S, C, NS>;
+  using Sm = LaSimtSmem<S, C, NS, MD>;
   Sm& sm = *reinterpret_cast<Sm*>(la_smem);
   constexpr int TN = NS / 4;              // threads across the columns
-  static_assert(256 / TN * 8 >= kLaMaxDim && C % 32 == 0, "thread tiles must cover the state");
+  constexpr int MR = MD * TN / 256;       // rows of the state per thread
+  static_assert(MR >= 2 && C % 32 == 0, "thread tiles must cover the state");
   constexpr int TR = C / (256 / TN);      // rows of o per thread
   const int role = blockIdx.y;
   const LaPass<S>& p = a.p[role];
@@ -138,26 +150,102 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
   const T* w = static_cast<const T*>(p.w) + b * p.ws[0] + h * p.ws[2] + n0;
   const S* g = a.g + b * a.gs[0] + h * a.gs[2];
 
-  S st[8][4];
+  S st[MR][4];
   {
     const S* src = nullptr;
     bool tr = false;
     if (!STATES_ONLY && ord > 0) src = a.seg + ((int64_t)(role * a.nseg + ord) * BH + bh) * a.seg_stride;
     else if (!STATES_ONLY && p.init) { src = p.init + bh * M * N; tr = p.state_t; }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < MR; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int m = tm * 8 + i, n = n0 + tn * 4 + j;
+        const int m = tm * MR + i, n = n0 + tn * 4 + j;
         st[i][j] = (src && m < M && n < N) ? src[tr ? (int64_t)n * M + m : (int64_t)m * N + n] : (S)0;
       }
   }
   double seg_log = 0.0;
   const int M4 = (M + 3) & ~3;
+  auto chunk_of = [&](int64_t ci) { return p.reverse ? c1 - 1 - (ci - c0) : ci; };
+  auto valid = [&](int64_t c) { return (int)max((int64_t)0, min((int64_t)C, len - c * C)); };
+  // a chunk's decays, by one warp, a chunk ahead of their use
+  auto decays = [&](int64_t ci, int buf) {
+    const int64_t c = chunk_of(ci);
+    la_running_logs<S, C>(sm.G[buf], g, a.gs[1], c * C, valid(c), lane);
+    __syncwarp();
+    const double E = sm.G[buf][C - 1];
+    for (int i = lane; i < C; i += 32) {
+      const S up = la_exp((S)sm.G[buf][i]), down = la_exp((S)(E - sm.G[buf][i]));
+      sm.win[buf][i] = p.reverse ? down : up;
+      sm.wout[buf][i] = (p.reverse ? up : down) * p.pz;
+    }
+  };
+  // a warp takes whole rows of the operands: a lane every 32nd value, the next chunk's on their way to
+  // registers while this one is worked on
+  constexpr int RW = C / 8, ZW = NS / 32;
+  constexpr int XW = MD / 32;
+  S rx[RW][XW], ry[RW][XW], rz[RW][ZW];
+  const int warp = tid >> 5;
+  auto fetch = [&](int64_t ci) {
+    const int64_t c = chunk_of(ci), t0 = c * C;
+    const int n = valid(c);
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+      const int r = warp + 8 * i;
+#pragma unroll
+      for (int k = 0; k < XW; ++k) {
+        const int m = lane + 32 * k;
+        const bool ok = r < n && m < M;
+        if (!STATES_ONLY) rx[i][k] = ok ? la_load<S, T>(x + (t0 + r) * p.xs[1] + m) : (S)0;
+        ry[i][k] = ok ? la_load<S, T>(y + (t0 + r) * p.ys[1] + m) : (S)0;
+      }
+#pragma unroll
+      for (int k = 0; k < ZW; ++k) {
+        const int q = lane + 32 * k;
+        rz[i][k] = (r < n && q < nw) ? la_load<S, T>(z + (t0 + r) * p.zs[1] + q) : (S)0;
+      }
+    }
+  };
+  if (c0 < c1) {
+    fetch(c0);
+    if (warp == 7) decays(c0, 0);
+  }
   for (int64_t ci = c0; ci < c1; ++ci) {
-    const int64_t c = p.reverse ? c1 - 1 - (ci - c0) : ci;
-    const int64_t t0 = c * C;
-    const int n = (int)max((int64_t)0, min((int64_t)C, len - t0));   // valid tokens
+    const int64_t c = chunk_of(ci), t0 = c * C;
+    const int n = valid(c), buf = (int)((ci - c0) & 1);
+    __syncthreads();   // everything of the previous chunk has been read
+    if (n > 0) {
+#pragma unroll
+      for (int i = 0; i < RW; ++i) {
+        const int r = warp + 8 * i;
+#pragma unroll
+        for (int k = 0; k < XW; ++k) {
+          if (!STATES_ONLY) sm.x[r][lane + 32 * k] = rx[i][k];
+          sm.y[r][lane + 32 * k] = ry[i][k];
+        }
+#pragma unroll
+        for (int k = 0; k < ZW; ++k) sm.z[r][lane + 32 * k] = rz[i][k];
+      }
+      if (!STATES_ONLY) {
+#pragma unroll
+          for (int i = 0; i < MR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sm.s[tm * MR + i][tn * 4 + j] = st[i][j];
+        if (p.bounds) {
+          S* dst = p.bounds + (bh * nchunk + c) * M * N;
+#pragma unroll
+          for (int i = 0; i < MR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int m = tm * MR + i, q = n0 + tn * 4 + j;
+              if (m < M && q < N) dst[(int64_t)m * N + q] = st[i][j];
+            }
+        }
+      }
+    }
+    if (ci + 1 < c1) fetch(ci + 1);
+    __syncthreads();
+    if (warp == 7 && ci + 1 < c1) decays(ci + 1, buf ^ 1);
     if (n == 0) {            // behind the sequence: zeros come out, the state stays
       if (!STATES_ONLY && p.o) {
         for (int i = tid; i < C * nw; i += 256) {
@@ -169,62 +257,20 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
       }
       continue;
     }
-    __syncthreads();
-    for (int i = tid; i < C * M4; i += 256) {
-      const int r = i / M4, m = i % M4;
-      const bool ok = r < n && m < M;
-      if (!STATES_ONLY) sm.x[r][m] = ok ? la_load<S, T>(x + (t0 + r) * p.xs[1] + m) : (S)0;
-      sm.y[r][m] = ok ? la_load<S, T>(y + (t0 + r) * p.ys[1] + m) : (S)0;
-    }
-    for (int i = tid; i < C * NS; i += 256) {
-      const int r = i / NS, q = i % NS;
-      sm.z[r][q] = (r < n && q < nw) ? la_load<S, T>(z + (t0 + r) * p.zs[1] + q) : (S)0;
-    }
-    if (tid < 32) {
-      la_running_logs<S, C>(sm.G, g, a.gs[1], t0, n, lane);
-      __syncwarp();
-      const double E = sm.G[C - 1];
-      for (int i = lane; i < C; i += 32) {
-        const S up = la_exp((S)sm.G[i]), down = la_exp((S)(E - sm.G[i]));
-        sm.win[i] = p.reverse ? down : up;
-        sm.wout[i] = p.reverse ? up : down;
-      }
-    }
-    if (!STATES_ONLY) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int m = tm * 8 + i;
-          if (m < kLaMaxDim) sm.s[m][tn * 4 + j] = st[i][j];
-        }
-      if (p.bounds) {
-        S* dst = p.bounds + (bh * nchunk + c) * M * N;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int m = tm * 8 + i, q = n0 + tn * 4 + j;
-            if (m < M && q < N) dst[(int64_t)m * N + q] = st[i][j];
-          }
-      }
-    }
-    __syncthreads();
-    const double E = sm.G[C - 1];
+    const double* const G = sm.G[buf];
+    const double E = G[C - 1];
     if (!STATES_ONLY) {
       {   // scores inside the chunk with their decays: a CR x CS block per thread, strided over the rows
         constexpr int TS = 16, CR = C / (256 / TS), CS = C / TS;
         const int ts = tid % TS, tr = tid / TS;
         S acc[CR][CS] = {};
+#pragma unroll 4
         for (int m = 0; m < M4; m += 4) {
           S xv[CR][4], yv[CS][4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int i = 0; i < CR; ++i) la_get4(xv[i], &sm.x[tr * CR + i][m]);
 #pragma unroll
-            for (int i = 0; i < CR; ++i) xv[i][k] = sm.x[tr * CR + i][m + k];
-#pragma unroll
-            for (int j = 0; j < CS; ++j) yv[j][k] = sm.y[ts + TS * j][m + k];
-          }
+          for (int j = 0; j < CS; ++j) la_get4(yv[j], &sm.y[ts + TS * j][m]);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -237,35 +283,50 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
 #pragma unroll
           for (int j = 0; j < CS; ++j) {
             const int t = tr * CR + i, s = ts + TS * j;
-            const bool on = p.reverse ? s >= t : s <= t;
-            const double d = p.reverse ? sm.G[s] - sm.G[t] : sm.G[t] - sm.G[s];
-            sm.p[t][s] = on ? acc[i][j] * la_exp((S)d) * p.pz : (S)0;
+            const S w = la_exp((S)(p.reverse ? G[s] - G[t] : G[t] - G[s])) * p.pz;
+            sm.p[t][s] = (p.reverse ? s >= t && s < n : s <= t) ? acc[i][j] * w : (S)0;
           }
       }
-      __syncthreads();
-      // o: TR rows (strided) x 4 columns per thread
+      // o: TR rows x 4 columns per thread
       S intra[TR][4] = {}, inter[TR][4] = {};
-      for (int m = 0; m < M; ++m) {
-        S sv[4];
+#pragma unroll 2
+      for (int m = 0; m < M4; m += 4) {   // rows of the state from M on are zero
+        S sv[4][4], xv[TR][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sv[j] = sm.s[m][tn * 4 + j];
+        for (int k = 0; k < 4; ++k) la_get4(sv[k], &sm.s[m + k][tn * 4]);
 #pragma unroll
-        for (int i = 0; i < TR; ++i) {
-          const S xv = sm.x[tm * TR + i][m];
+        for (int i = 0; i < TR; ++i) la_get4(xv[i], &sm.x[tm * TR + i][m]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) inter[i][j] += xv * sv[j];
-        }
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < TR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) inter[i][j] += xv[i][k] * sv[k][j];
       }
-      const int s_lo = p.reverse ? tm * TR : 0, s_hi = p.reverse ? C : tm * TR + TR;
+      __syncthreads();
+      // tokens before (mirrored: behind) all of the thread's rows, then the few among them: a masked token is not read,
+      // 0 * inf would be NaN
+      const int s_lo = p.reverse ? tm * TR + TR : 0, s_hi = p.reverse ? n : tm * TR;
+#pragma unroll 4
       for (int s = s_lo; s < s_hi; ++s) {
         S zv[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) zv[j] = sm.z[s][tn * 4 + j];
+        la_get4(zv, &sm.z[s][tn * 4]);
 #pragma unroll
         for (int i = 0; i < TR; ++i) {
-          const int t = tm * TR + i;
-          if (p.reverse ? s < t : s > t) continue;   // a masked token is not read: 0 * inf would be NaN
-          const S pv = sm.p[t][s];
+          const S pv = sm.p[tm * TR + i][s];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) intra[i][j] += pv * zv[j];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < TR; ++k) {
+        const int s = tm * TR + k;
+        S zv[4];
+        la_get4(zv, &sm.z[s][tn * 4]);
+#pragma unroll
+        for (int i = 0; i < TR; ++i) {
+          if (p.reverse ? k < i || s >= n : k > i) continue;
+          const S pv = sm.p[tm * TR + i][s];
 #pragma unroll
           for (int j = 0; j < 4; ++j) intra[i][j] += pv * zv[j];
         }
@@ -274,7 +335,7 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
       for (int i = 0; i < TR; ++i) {
         const int r = tm * TR + i;
         const int64_t t = t0 + r;
-        const S win = sm.win[r];
+        const S win = sm.win[buf][r];
         S d0 = 0, d1 = 0;
         const int64_t at = ((b * a.T + t) * a.H + h) * N + n0;
 #pragma unroll
@@ -309,21 +370,28 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
     {   // the state moves on by one chunk
       const S dec = la_exp((S)E);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < MR; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) st[i][j] *= dec;
-      if (tm * 8 < M4) {
-        for (int s = 0; s < n; ++s) {
-          const S wv = sm.wout[s] * p.pz;
-          S zv[4];
+      if (tm * MR < M4) {
+#pragma unroll 4
+        for (int s = 0; s < C; ++s) {   // tokens from n on are zero
+          const S wv = sm.wout[buf][s];
+          S zv[4], yv[MR];
+          la_get4(zv, &sm.z[s][tn * 4]);
+          if constexpr (MR >= 4) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) zv[j] = sm.z[s][tn * 4 + j] * wv;
+            for (int i = 0; i < MR; i += 4) la_get4(*reinterpret_cast<S(*)[4]>(&yv[i]), &sm.y[s][tm * MR + i]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const S yv = sm.y[s][tm * 8 + i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) st[i][j] += yv * zv[j];
+            for (int i = 0; i < MR; ++i) yv[i] = sm.y[s][tm * MR + i];
           }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) zv[j] *= wv;
+#pragma unroll
+          for (int i = 0; i < MR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) st[i][j] += yv[i] * zv[j];
         }
       }
     }
@@ -335,10 +403,10 @@ __global__ void __launch_bounds__(256) la_simt_kernel(const LaArgs<S> a) {
   else if (p.fin && ord == a.nseg - 1) { dst = p.fin + bh * M * N; tr = p.state_t; }
   if (dst) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < MR; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int m = tm * 8 + i, q = n0 + tn * 4 + j;
+        const int m = tm * MR + i, q = n0 + tn * 4 + j;
         if (m < M && q < N) dst[tr ? (int64_t)q * M + m : (int64_t)m * N + q] = st[i][j];
       }
   }

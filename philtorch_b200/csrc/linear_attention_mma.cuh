@@ -23,6 +23,12 @@ __device__ __forceinline__ uint32_t la_pack(float lo, float hi) {   // {lo, hi} 
 __device__ __forceinline__ float la_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float la_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// exp of a difference of log decays given in units of log 2; results below the normal range are zero
+__device__ __forceinline__ float la_exp2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ void la_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -73,8 +79,8 @@ struct LaMmaSmem {
   static constexpr int C = kLaMmaChunk;
   static constexpr int X = C * MP * 2, Z = C * NP * 2, STAGE = 2 * X + Z;   // x, y, z
   static constexpr int P = C * C * 2;
-  // after the stages: P, G (double), win, wout, row and column sums of the decay's gradient
-  static constexpr int MISC = C * 8 + 2 * C * 4 + (4 + 4 + 1) * C * 4;
+  // after the stages: P, G (double), win, wout, row and column sums of the decay's gradient, G in two floats
+  static constexpr int MISC = C * 8 + 2 * C * 4 + (4 + 4 + 1 + 2) * C * 4;
   static int bytes(int stages, bool dots) { return stages * STAGE + (dots ? Z : 0) + P + MISC; }
 };
 
@@ -118,6 +124,8 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
   float* const cols = wout + C;        // [4][C]
   float* const ext = cols + 4 * C;     // [4][C]: each warp's share of w.o from the entering state
   float* const rows = ext + 4 * C;     // [C]
+  float* const Gh = rows + C;          // [C], [C]: the running sums in units of log 2, in two floats (what one float loses of
+  float* const Gl = Gh + C;            //   them would be lost to the difference of two tokens behind a strong decay)
 
   float st[NJ][MT][4];
   {
@@ -191,6 +199,9 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
         const float up = expf((float)G[i]), down = expf((float)(E - G[i]));
         win[i] = rev ? down : up;
         wout[i] = (rev ? up : down) * p.pz;
+        const double in = (rev ? -G[i] : G[i]) * 1.4426950408889634;
+        Gh[i] = (float)in;
+        Gl[i] = (float)(in - (double)Gh[i]);
       }
     }
     if (VEC) {
@@ -215,7 +226,7 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
       }
       {   // scores of the rows 16 warp .. 16 warp + 15
         float sc[8][4] = {};
-#pragma unroll
+#pragma unroll 1
         for (int kk = 0; kk < MP / 16; ++kk) {
           uint32_t av[4];
           la_ldm(av, la_at<MP>(sx, 16 * warp + (lane & 15), 2 * kk + (lane >> 4)));
@@ -229,17 +240,18 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
             }
         }
         const int r0 = 16 * warp + g4;
-        const double G0 = G[r0], G1 = G[r0 + 8];
-        float wt[8][4];
+        const float2 own0 = make_float2(Gh[r0], Gl[r0]), own1 = make_float2(Gh[r0 + 8], Gl[r0 + 8]);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (rev ? j >= 2 * warp : j < 2 * warp + 2) {
+            const float2 gh = *reinterpret_cast<const float2*>(Gh + 8 * j + 2 * t4), gl = *reinterpret_cast<const float2*>(Gl + 8 * j + 2 * t4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int s = 8 * j + 2 * t4 + (e & 1), t = r0 + (e >> 1) * 8;
-              const double d = (e >> 1 ? G1 : G0) - G[s];
-              wt[j][e] = (rev ? s >= t : s <= t) ? expf((float)(rev ? -d : d)) * p.pz : 0.f;
-              sc[j][e] = wt[j][e] != 0.f ? sc[j][e] * wt[j][e] : 0.f;
+              const float2 own = e >> 1 ? own1 : own0;
+              const float d = (own.x - (e & 1 ? gh.y : gh.x)) + (own.y - (e & 1 ? gl.y : gl.x));
+              const float w = la_exp2(d) * p.pz;   // (mirrored: the sums are stored negated)
+              sc[j][e] = (rev ? s >= t && s < n : s <= t) ? sc[j][e] * w : 0.f;
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -249,7 +261,7 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
           }
         if (dots) {   // pairs (t, s) inside the chunk: weight * (x.y)(w.z), summed over rows and over columns
           float s2[8][4] = {};
-#pragma unroll
+#pragma unroll 1
           for (int kk = 0; kk < NP / 16; ++kk) {
             uint32_t av[4];
             la_ldm(av, la_at<NP>(s_w, 16 * warp + (lane & 15), 2 * kk + (lane >> 4)));
@@ -341,7 +353,7 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
           if (t4 == 0) { ext[warp * C + 16 * i + g4] = d0; ext[warp * C + 16 * i + g4 + 8] = d1; }
         }
       }
-#pragma unroll
+#pragma unroll 1
       for (int kk = 0; kk < 4; ++kk) {   // the chunk's own tokens
         uint32_t zv[NJ][4];
 #pragma unroll
@@ -409,7 +421,7 @@ __global__ void __launch_bounds__(128) la_mma_kernel(const LaArgs<float> a, cons
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) st[j][i][e] *= dec;
-#pragma unroll
+#pragma unroll 1
       for (int kk = 0; kk < 4; ++kk) {
         const float w0 = wout[16 * kk + 2 * t4], w1 = wout[16 * kk + 2 * t4 + 1];
         const float w2 = wout[16 * kk + 2 * t4 + 8], w3 = wout[16 * kk + 2 * t4 + 9];

@@ -99,12 +99,6 @@ __device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t (&r)[8]) {
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-// exp of a difference of log decays given in units of log 2; results below the normal range are zero
-__device__ __forceinline__ float tc_exp2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap* map, int d, int t, int h, int b, uint64_t* bar) {
@@ -136,11 +130,11 @@ constexpr uint32_t kTcDescHi = (2u << 29) | (1u << 14) | (1024 >> 4);
 __device__ __forceinline__ uint32_t tc_desc(uint32_t tile) { return ((uint32_t)(kTcPanel >> 4) << 16) | (tile >> 4); }   // low word
 // K / 16 products over one tile: operand a from shared memory (K- or MN-major) or, as packed columns, from tensor memory
 enum TcOperand { kKMajor, kMnMajor, kTmem };
-template <TcOperand A, TcOperand B, int STEPS>
-__device__ __forceinline__ void tc_products(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool fresh) {
+template <TcOperand A, TcOperand B>
+__device__ __forceinline__ void tc_products(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool fresh, int steps = 8) {
   constexpr uint32_t kRow = 2, kDown = 2048 >> 4, kOver = kTcPanel >> 4;
 #pragma unroll 1
-  for (int k0 = 0; k0 < STEPS; k0 += 4) {   // the 64 columns of a panel, or 64 rows
+  for (int k0 = 0; k0 < steps; k0 += 4) {   // the 64 columns of a panel, or 64 rows
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       const uint64_t db = ((uint64_t)kTcDescHi << 32) | (b + kk * (B == kKMajor ? kRow : kDown));
@@ -194,10 +188,10 @@ __device__ __forceinline__ void tc_logs(float* Gs, TcFactors* f, const float (&r
   if (lane == 0) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      f->before[k] = tc_exp2((float)run);
-      f->over[k] = tc_exp2((float)end[k]);
+      f->before[k] = la_exp2((float)run);
+      f->over[k] = la_exp2((float)end[k]);
       run += end[k];
-      f->after[k] = tc_exp2((float)(E - run));
+      f->after[k] = la_exp2((float)(E - run));
     }
     // 1 + (e^x - 1) keeps its error relative to the decay's distance from one
     const float x = (float)(E * 0.69314718055994531), q = expm1f(x), one = 1.f + q;
@@ -332,17 +326,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
       constexpr uint32_t kScD = tc_idesc(128, 128, false, false), kOD = tc_idesc(128, 64, false, true),
                          kUD = tc_idesc(128, 64, true, true);
       const uint32_t Zw = tc_desc(base + L.zw), S = tc_desc(base + L.s);
+      const int steps = M > 64 ? 8 : 4;   // of 16 channels of x and y
       auto scores = [&](int i) {
         const int s = i % sxy, sz = i & 1;
         const uint32_t X = tc_desc(base + s * 4 * kTcPanel), Y = X + (2 * kTcPanel >> 4);
         wait_warp(xy_full + s, (i / sxy) & 1);
         tc_after();
-        if (one) tc_products<kKMajor, kKMajor, 8>(tm + kSC, X, Y, kScD, true);
+        if (one) tc_products<kKMajor, kKMajor>(tm + kSC, X, Y, kScD, true, steps);
         if (DOTS) {
           const uint32_t Z = tc_desc(base + L.z + sz * 2 * kTcPanel);
           wait_warp(zw_full + sz, (i / 2) & 1);
           tc_after();
-          if (one) tc_products<kKMajor, kKMajor, 4>(tm + kSC2, Z + (kTcPanel >> 4), Z, kScD, true);
+          if (one) tc_products<kKMajor, kKMajor>(tm + kSC2, Z + (kTcPanel >> 4), Z, kScD, true, 4);
         }
         if (one) tc_commit(b_sc);
       };
@@ -357,7 +352,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         tc_after();
 #pragma unroll 1
         for (int term = nu - 1; term >= 0; --term)   // smallest first
-          if (one) tc_products<kMnMajor, kMnMajor, 8>(tm + kU, Y, Zw + term * (kTcPanel >> 4), kUD, term == nu - 1);
+          if (one) tc_products<kMnMajor, kMnMajor>(tm + kU, Y, Zw + term * (kTcPanel >> 4), kUD, term == nu - 1);
         if (one) tc_commit(b_u);
         if (!STATES_ONLY) {
           wait_warp(b_s, i & 1);
@@ -365,14 +360,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
           tc_after();
 #pragma unroll 1
           for (int term = ns - 1; term >= 0; --term)
-            if (one) tc_products<kKMajor, kMnMajor, 8>(tm + kOI + at, X, S + term * (kTcPanel >> 4), kOD, term == ns - 1);
+            if (one) tc_products<kKMajor, kMnMajor>(tm + kOI + at, X, S + term * (kTcPanel >> 4), kOD, term == ns - 1, steps);
           if (one) tc_commit(b_oi);
         }
         if (one) tc_commit(xy_empty + s);
         if (!STATES_ONLY) {
           wait_warp(b_p, i & 1);
           tc_after();
-          if (one) tc_products<kTmem, kMnMajor, 8>(tm + kO + at, tm + kP, Z, kOD, true);
+          if (one) tc_products<kTmem, kMnMajor>(tm + kO + at, tm + kP, Z, kOD, true);
           if (one) tc_commit(b_o);
         }
         if (one) tc_commit(zw_empty + sz);
@@ -413,8 +408,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         const float2 whole = make_float2(G[32 * quad + 31], G[C + 32 * quad + 31]);
         row_own = make_float2(G[row], G[C + row]);
         // from the token to its block's end, and from the block's start to it
-        const float to_end = tc_exp2(rev ? (row_own.x - whole.x) + (row_own.y - whole.y) : (whole.x - row_own.x) + (whole.y - row_own.y));
-        const float to_start = tc_exp2(rev ? -row_own.x : row_own.x);
+        const float to_end = la_exp2(rev ? (row_own.x - whole.x) + (row_own.y - whole.y) : (whole.x - row_own.x) + (whole.y - row_own.y));
+        const float to_start = la_exp2(rev ? -row_own.x : row_own.x);
         row_col = rev ? to_start : to_end;
         row_mine = rev ? to_end : to_start;
         row_win = row_mine * (rev ? f.after[quad] : f.before[quad]) * p.po;
@@ -514,7 +509,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
             for (int j = 0; j < 16; j += 2) {
               const float2 e = ((own_hi - TcPair(*reinterpret_cast<const uint64_t*>(G + q * 16 + j))) +
                                 (own_lo - TcPair(*reinterpret_cast<const uint64_t*>(G + C + q * 16 + j)))).get();
-              const float2 w = (tc_pair(v[j], v[j + 1]) * tc_pair(tc_exp2(e.x), tc_exp2(e.y))).get();
+              const float2 w = (tc_pair(v[j], v[j + 1]) * tc_pair(la_exp2(e.x), la_exp2(e.y))).get();
               v[j] = on >> j & 1 ? __float_as_uint(w.x) : 0u;
               v[j + 1] = on >> (j + 1) & 1 ? __float_as_uint(w.y) : 0u;
             }
@@ -603,7 +598,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
       const float* const G = Gs + (i & 1) * 2 * C;
       const TcFactors& f = fac[i & 1];
       const float2 own = make_float2(G[row], G[C + row]), whole = make_float2(G[32 * quad + 31], G[C + 32 * quad + 31]);
-      wt = (rev ? tc_exp2(-own.x) * f.before[quad] : tc_exp2((whole.x - own.x) + (whole.y - own.y)) * f.after[quad]) * p.pz;
+      wt = (rev ? la_exp2(-own.x) * f.before[quad] : la_exp2((whole.x - own.x) + (whole.y - own.y)) * f.after[quad]) * p.pz;
       dec_now = make_float2(f.dec[0], f.dec[1]);
       arrive_warp(lg_empty + (i & 1));
     };
