@@ -201,7 +201,7 @@ static bool la_tc_map(LaTcMap* m, const void* base, const int64_t* st, int64_t B
 }
 
 // The tcgen05 kernels take every size whose operands the TMA unit can address; the mma.sync kernels the others
-// (odd or unaligned head sizes).  B=1, H=4, D=64, T=256: 31.6 us on mma.sync, XXX us here.
+// (odd or unaligned head sizes).  B=1, H=4, D=64, T=256: 31.6 us on mma.sync, 11.4 us here.
 static bool la_tc_setup(LaTcArgs* k, const LaArgs<float>& a, int roles) {
   if (a.T < 1 || a.T > 0x7fffffffll || !la_mma_vec(a, roles)) return false;
   for (int r = 0; r < roles; ++r) {
@@ -295,19 +295,26 @@ static int la_run(LaArgs<S>& a, LaTcArgs* k, LaPath path, int roles, const LaPla
     bool dots = false;
     for (int r = 0; r < roles; ++r) dots = dots || a.p[r].dots;
     const bool vec = la_mma_vec(a, roles);
-    if (std::max(a.p[0].M, a.p[0].N) <= 64)
-      return vec ? la_mma_run<64, true>(a, roles, dots, st) : la_mma_run<64, false>(a, roles, dots, st);
-    return vec ? la_mma_run<128, true>(a, roles, dots, st) : la_mma_run<128, false>(a, roles, dots, st);
-  } else {
-    int most = 0;   // channels of x and y
-    for (int r = 0; r < roles; ++r) most = std::max(most, a.p[r].M);
-    return most <= 64 ? la_simt_run<T, S, 64>(a, roles, st) : la_simt_run<T, S, 128>(a, roles, st);
+    if (path == kLaMma) {
+      if (std::max(a.p[0].M, a.p[0].N) <= 64)
+        return vec ? la_mma_run<64, true>(a, roles, dots, st) : la_mma_run<64, false>(a, roles, dots, st);
+      return vec ? la_mma_run<128, true>(a, roles, dots, st) : la_mma_run<128, false>(a, roles, dots, st);
+    }
   }
+  int most = 0;   // channels of x and y
+  for (int r = 0; r < roles; ++r) most = std::max(most, a.p[r].M);
+  return most <= 64 ? la_simt_run<T, S, 64>(a, roles, st) : la_simt_run<T, S, 128>(a, roles, st);
 }
+
+// One chunk of the CUDA-core kernels: as fast there as on the tensor cores (B=1, H=4, D=64, T=1: 9.2 against 11.4 us;
+// T=64: 16.1 against 10.3), and where an output is a sum of a few terms, the rounding of their weights to bfloat16
+// would not average out.
+constexpr int64_t kLaShort = LaGeom<float>::C;
 
 template <class T, class S>
 static LaPath la_path(LaTcArgs* k, const LaArgs<S>& a, int roles) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) return la_tc_setup(k, a, roles) ? kLaTc : kLaMma;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    if (a.T > kLaShort) return la_tc_setup(k, a, roles) ? kLaTc : kLaMma;
   return kLaSimt;
 }
 
@@ -470,7 +477,7 @@ int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, in
   const LaSize z = {B, T, H, Dk, Dv};
   const int roles = backward ? 3 : 1;
   if (dtype == PTB_F64) return la_plan_of<double>(kLaSimt, z, roles, decay_grad).total;
-  if (dtype != PTB_BF16) return la_plan_of<float>(kLaSimt, z, roles, decay_grad).total;
+  if (dtype != PTB_BF16 || T <= kLaShort) return la_plan_of<float>(kLaSimt, z, roles, decay_grad).total;
   // which of the tensor-core kernels run depends on the operands' alignment too: room for either
   return std::max(la_mma_plan(z, roles, decay_grad).total, la_tc_plan(z, roles, decay_grad).total);
 }
