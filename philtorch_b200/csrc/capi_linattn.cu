@@ -19,10 +19,12 @@ struct LaPlan {
 
 // Few (batch, head) pairs: the time axis is cut into segments that run side by side.  Their entering states
 // come from a first pass that only forms states (about half the work of a chunk), so a cut into n segments takes
-// about 1.5 / n of the time plus two launches: it pays from n = 2 on, where the row has chunks to spare.
-static void la_cut(int64_t ctas, int64_t nchunk, int64_t room, int* nseg, int* seg_chunks) {
+// about 1.5 / n of the time plus two launches.  least: the n from which it pays.  Measured: 2 on the CUDA cores (float32
+// training step (2, 509, 3, 33/65): 137 -> 42 us per direction); on the tensor cores two segments of 64 (batch,
+// head, slice) CTAs take 89 us against 80 uncut (2, 4096, 16, 128), so 3.
+static void la_cut(int64_t ctas, int64_t nchunk, int64_t room, int64_t least, int* nseg, int* seg_chunks) {
   int64_t n = ctas > 0 ? std::min(room / ctas, nchunk / 2) : 1;
-  if (n < 2 || nchunk < 8) n = 1;
+  if (n < least || nchunk < 8) n = 1;
   const int64_t per = n > 1 ? (nchunk + n - 1) / n : std::max<int64_t>(nchunk, 1);
   *seg_chunks = (int)per;
   *nseg = n > 1 ? (int)((nchunk + per - 1) / per) : 1;
@@ -40,7 +42,7 @@ static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int wi
   const int64_t slices = roles == 1 ? over_v : 2 * over_k + over_v;   // of o; of dq, dk and dv
   l.nchunk = (z.T + C - 1) / C;
   const int64_t BH = z.B * z.H;
-  la_cut(BH * slices, l.nchunk, kLaSms * per_sm, &l.nseg, &l.seg_chunks);
+  la_cut(BH * slices, l.nchunk, kLaSms * per_sm, C == kTcChunk ? 3 : 2, &l.nseg, &l.seg_chunks);
   l.seg_stride = align_up(mn, 64);
   l.bound_elems = mn;
   int64_t at = 0;
