@@ -319,6 +319,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         tc_tma(Z, &k.z[role].map, n0, t0, (int)h * k.z[role].hmul, (int)b * k.z[role].bmul, zw_full + sz);
         if (DOTS) tc_tma(Z + kTcPanel, &k.w[role].map, n0, t0, (int)h * k.w[role].hmul, (int)b * k.w[role].bmul, zw_full + sz);
       }
+      // nothing is on its way when the CTA ends, whatever its waits came to
+      for (int i = max(0, count - 2); i < count; ++i) {
+        if (i >= count - sxy && !mbar_wait_bounded(xy_full + i % sxy, (i / sxy) & 1, k.wait_cycles / 2)) *gave_up = 1;
+        if (!mbar_wait_bounded(zw_full + (i & 1), (i / 2) & 1, k.wait_cycles / 2)) *gave_up = 1;
+      }
     }
   } else if (warp == 16) {
     {   // products: the warp stays together (operands in uniform registers), one thread issues
@@ -373,6 +378,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         if (one) tc_commit(zw_empty + sz);
         if (!STATES_ONLY && i + 1 < count) scores(i + 1);
       }
+      if (count > 0 && !mbar_wait_bounded(zw_empty + ((count - 1) & 1), ((count - 1) / 2) & 1, k.wait_cycles / 2)) *gave_up = 1;
     }
   } else if (warp == 18) {   // decays
     float raw[4], next[4];
