@@ -29,7 +29,6 @@ __all__ = ["LinearAttention", "MAX_HEAD_DIM"]
 MAX_HEAD_DIM = 128
 _CODES = {torch.float32: _lib.PTB_F32, torch.float64: _lib.PTB_F64, torch.float16: _lib.PTB_F16,
           torch.bfloat16: _lib.PTB_BF16}
-_I3, _I2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
 
 
 def state_dtype(dtype: torch.dtype) -> torch.dtype:
@@ -37,14 +36,21 @@ def state_dtype(dtype: torch.dtype) -> torch.dtype:
     return torch.float64 if dtype == torch.float64 else torch.float32
 
 
-def _strides3(t: Tensor):
-    a, b, c, _ = t.stride()
-    return _I3(a, b, c)
+_stride_arrays: dict = {}
 
 
-def _strides2(t: Tensor):
-    a, b, _ = t.stride()
-    return _I2(a, b)
+def _array(strides: tuple):
+    """The strides as a ctypes array (kept by value: a program's tensors have few different ones)."""
+    a = _stride_arrays.get(strides)
+    if a is None:
+        if len(_stride_arrays) > 4096:
+            _stride_arrays.clear()
+        a = _stride_arrays[strides] = (ctypes.c_int64 * len(strides))(*strides)
+    return a
+
+
+def _outer_strides(t: Tensor):
+    return _array(t.stride()[:-1])
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -94,7 +100,7 @@ def _check(q: Tensor, k: Tensor, v: Tensor, g: Tensor, init: Optional[Tensor], l
 
 
 def _decay_strides(g: Tensor):
-    return _I3(0, 0, g.stride(0)) if g.dim() == 1 else _I3(*g.stride())
+    return _array((0, 0, g.stride(0)) if g.dim() == 1 else g.stride())
 
 
 _ws_bytes: dict = {}
@@ -140,8 +146,8 @@ def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state, wide
     o = (log_decay if wide else v).new_empty((B, T, H, Dv))   # wide: in the sums' type, for a normalisation that follows
     state = log_decay.new_empty((B, H, Dk, Dv) if want_state else (0,))
     if B and H and (T or want_state):
-        _lib.call(lib.ptb_linear_attention_fwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides3(q), ptr(k), _strides3(k),
-                  ptr(v), _strides3(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(o),
+        _lib.call(lib.ptb_linear_attention_fwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k), _outer_strides(k),
+                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(o),
                   int(o.dtype != v.dtype), ptr(state) if want_state else None, ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 0, 0))
     return o, state
 
@@ -163,9 +169,9 @@ def _linear_attention_bwd(q, k, v, log_decay, init, lengths, scale, grad_o, grad
     ginit = log_decay.new_empty((B, H, Dk, Dv) if need_init else (0,))
     if B and H:
         opt = lambda t, need: ptr(t) if need else None   # noqa: E731
-        _lib.call(lib.ptb_linear_attention_bwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _strides3(q), ptr(k), _strides3(k),
-                  ptr(v), _strides3(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(grad_o),
-                  _strides3(grad_o), ptr(grad_state), opt(gq, need_q), opt(gk, need_k), opt(gv, need_v),
+        _lib.call(lib.ptb_linear_attention_bwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k), _outer_strides(k),
+                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(grad_o),
+                  _outer_strides(grad_o), ptr(grad_state), opt(gq, need_q), opt(gk, need_k), opt(gv, need_v),
                   opt(gg, need_decay), int(log_decay.dim() == 3), opt(ginit, need_init),
                   ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 1, int(need_decay)))
     else:
@@ -214,10 +220,10 @@ def _linear_attention_step(q, k, v, log_decay, state, scale):
     q, k, v = _rows(q), _rows(k), _rows(v)
     o = v.new_empty((B, H, Dv))
     if B and H:
-        gs = _I2(0, log_decay.stride(0)) if log_decay.dim() == 1 else _I2(*log_decay.stride())
-        _lib.launch(lib.ptb_linear_attention_step, dev, _code(q), B, H, Dk, Dv, ptr(q), _strides2(q), ptr(k),
-                    _strides2(k), ptr(v), _strides2(v), ptr(log_decay), gs, scale, ptr(state),
-                    _I2(*state.stride()[:2]), ptr(o))
+        gs = _array((0, log_decay.stride(0)) if log_decay.dim() == 1 else log_decay.stride())
+        _lib.launch(lib.ptb_linear_attention_step, dev, _code(q), B, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k),
+                    _outer_strides(k), ptr(v), _outer_strides(v), ptr(log_decay), gs, scale, ptr(state),
+                    _array(state.stride()[:2]), ptr(o))
         torch.autograd.graph.increment_version(state)
     return o
 

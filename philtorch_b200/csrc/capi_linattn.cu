@@ -216,8 +216,9 @@ static bool la_tc_setup(LaTcArgs* k, const LaArgs<float>& a, int roles) {
   return true;
 }
 
+// beside: may start while the kernel launched before it on the stream is running (it reads nothing that one writes)
 template <bool STATES_ONLY, bool DOTS>
-static int la_tc_launch(const LaTcArgs& k, int roles, cudaStream_t st) {
+static int la_tc_launch(const LaTcArgs& k, int roles, cudaStream_t st, bool beside = false) {
   static bool ready[kMaxDevices] = {};
   int dev = 0;
   PTB_CUDA(cudaGetDevice(&dev));
@@ -232,8 +233,17 @@ static int la_tc_launch(const LaTcArgs& k, int roles, cudaStream_t st) {
   }
   const int64_t grid = k.a.B * k.a.H * 2 * (STATES_ONLY ? k.a.nseg - (k.all_segments ? 0 : 1) : k.a.nseg);
   if (grid > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
-  la_tc_kernel<STATES_ONLY, DOTS><<<dim3((unsigned)grid, roles), kTcThreads, smem, st>>>(k);
-  PTB_CUDA(cudaGetLastError());
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, roles);
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = beside ? 1 : 0;
+  PTB_CUDA(cudaLaunchKernelEx(&cfg, la_tc_kernel<STATES_ONLY, DOTS>, k));
   return PTB_OK;
 }
 
@@ -265,7 +275,8 @@ static int la_tc_run(LaTcArgs& k, int roles, cudaStream_t st) {
     k.xy_stages = 2;
     return la_tc_launch<false, false>(k, roles, st);
   }
-  // the passes with dots, then the others (another use of the shared memory)
+  // the passes with dots, then, beside them, the others (another use of the shared memory).  One launch after the other
+  // leaves SMs idle twice: 96 and 48 CTAs at B=1, T=32768, H=4
   LaTcArgs part = k;
   int with = 0, without = 0;
   LaTcArgs plain = k;
@@ -281,7 +292,7 @@ static int la_tc_run(LaTcArgs& k, int roles, cudaStream_t st) {
   part.xy_stages = 1;
   plain.xy_stages = 2;
   if (int rc = la_tc_launch<false, true>(part, with, st)) return rc;
-  return without ? la_tc_launch<false, false>(plain, without, st) : PTB_OK;
+  return without ? la_tc_launch<false, false>(plain, without, st, true) : PTB_OK;
 }
 
 template <class T, class S>

@@ -220,7 +220,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   const int slice = (int)(blockIdx.x & 1);                       // two slots for slices: neighbours share x and y in L2
   const int ord = (int)((blockIdx.x >> 1) % seg_count);
   const int64_t bh = (blockIdx.x >> 1) / seg_count;
-  if (slice >= slices) return;
+  // The passes with dots let the next kernel on the stream start beside them as soon as all their CTAs run; that kernel
+  // may not end before them (what follows it reads the results of both), so its last CTA waits for their end.
+  if (DOTS && tid == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const bool last_cta = !STATES_ONLY && !DOTS && tid == 0 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+  if (slice >= slices) {
+    if (last_cta) asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   if (STATES_ONLY && k.all_segments && !p.fin && ord == a.nseg - 1) return;   // nobody asks for its end
   const int64_t b = bh / a.H, h = bh % a.H, BH = a.B * a.H;
   const int M = p.M, N = p.N, n0 = slice * kTcSlice;
@@ -254,6 +261,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
 
   if (base & 1023) {   // the swizzled tiles need it; dynamic shared memory starts that way without static arrays
     if (tid == 0 && k.status) atomicOr(k.status, kErrPipelineWait);
+    if (last_cta) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
   if (warp == 16) tc_alloc(tmem_slot, 512);
@@ -727,6 +735,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   tc_after();
   if (warp == 16) tc_dealloc(tm, 512);
   if (tid == 0 && *gave_up && k.status) atomicOr(k.status, kErrPipelineWait);
+  if (last_cta) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace ptb
