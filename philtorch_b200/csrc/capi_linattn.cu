@@ -217,7 +217,7 @@ static bool la_tc_setup(LaTcArgs* k, const LaArgs<float>& a, int roles) {
 }
 
 // beside: may start while the kernel launched before it on the stream is running (it reads nothing that one writes)
-template <bool STATES_ONLY, bool DOTS>
+template <bool STATES_ONLY, bool DOTS, bool WIDE = false>
 static int la_tc_launch(const LaTcArgs& k, int roles, cudaStream_t st, bool beside = false) {
   static bool ready[kMaxDevices] = {};
   int dev = 0;
@@ -227,7 +227,7 @@ static int la_tc_launch(const LaTcArgs& k, int roles, cudaStream_t st, bool besi
   {
     std::lock_guard<std::mutex> lock(init_mutex());
     if (!ready[dev]) {
-      PTB_CUDA(cudaFuncSetAttribute(la_tc_kernel<STATES_ONLY, DOTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      PTB_CUDA(cudaFuncSetAttribute(la_tc_kernel<STATES_ONLY, DOTS, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
       ready[dev] = true;
     }
   }
@@ -243,7 +243,7 @@ static int la_tc_launch(const LaTcArgs& k, int roles, cudaStream_t st, bool besi
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = beside ? 1 : 0;
-  PTB_CUDA(cudaLaunchKernelEx(&cfg, la_tc_kernel<STATES_ONLY, DOTS>, k));
+  PTB_CUDA(cudaLaunchKernelEx(&cfg, la_tc_kernel<STATES_ONLY, DOTS, WIDE>, k));
   return PTB_OK;
 }
 
@@ -273,7 +273,7 @@ static int la_tc_run(LaTcArgs& k, int roles, cudaStream_t st) {
   }
   if (!dots) {
     k.xy_stages = 2;
-    return la_tc_launch<false, false>(k, roles, st);
+    return a.p[0].wide ? la_tc_launch<false, false, true>(k, roles, st) : la_tc_launch<false, false>(k, roles, st);
   }
   // the passes with dots, then, beside them, the others (another use of the shared memory).  One launch after the other
   // leaves SMs idle twice: 96 and 48 CTAs at B=1, T=32768, H=4

@@ -208,7 +208,8 @@ __device__ __forceinline__ void tc_load_logs(float (&raw)[4], const float* g, in
   }
 }
 
-template <bool STATES_ONLY, bool DOTS>
+// WIDE: o holds float32 (its own kernel: what a kernel's loops hold of code has to stay in the instruction cache)
+template <bool STATES_ONLY, bool DOTS, bool WIDE>
 __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_constant__ LaTcArgs k) {
   extern __shared__ __align__(1024) unsigned char tc_smem[];
   constexpr int C = kTcChunk;
@@ -232,14 +233,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   const int64_t b = bh / a.H, h = bh % a.H, BH = a.B * a.H;
   const int M = p.M, N = p.N, n0 = slice * kTcSlice;
   const bool rev = p.reverse;
-  const int64_t len = la_length(a.lengths, b, a.T), nchunk = (a.T + C - 1) / C;
+  const int T = (int)a.T;   // below 2^31: the TMA unit's coordinates
+  const int len = (int)la_length(a.lengths, b, a.T), nchunk = (int)(((int64_t)T + C - 1) / C);
   const int seg = rev ? a.nseg - 1 - ord : ord;
-  const int64_t c0 = (int64_t)seg * a.seg_chunks, c1 = min(c0 + (int64_t)a.seg_chunks, nchunk);
+  const int c0 = seg * a.seg_chunks, c1 = min(c0 + a.seg_chunks, nchunk);
   // chunks with tokens: c0 .. c0 + count - 1, visited upwards or downwards
-  const int count = (int)max((int64_t)0, min(c1, (len + C - 1) / C) - c0);
+  const int count = max(0, min(c1, (int)(((int64_t)len + C - 1) / C)) - c0);
   const float* g = a.g + b * a.gs[0] + h * a.gs[2];
   auto chunk_of = [&](int i) { return c0 + (rev ? count - 1 - i : i); };
-  auto valid = [&](int64_t c) { return (int)min((int64_t)C, len - c * C); };
+  auto valid = [&](int c) { return min(C, len - c * C); };
 
   const int nu = k.nu[role], ns = k.ns[role], sxy = k.xy_stages;
   const LaTcSmem L(sxy, DOTS, 3, DOTS ? 3 : 1);
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     if (lane == 0) {   // loads
 #pragma unroll 1
       for (int i = 0; i < count; ++i) {
-        const int t0 = (int)(chunk_of(i) * C), s = i % sxy, sz = i & 1;
+        const int t0 = chunk_of(i) * C, s = i % sxy, sz = i & 1;
         if (i >= sxy) wait(xy_empty + s, (i / sxy - 1) & 1);
         const uint32_t X = base + s * 4 * kTcPanel, Y = X + 2 * kTcPanel;
         mbar_arrive_expect_tx(xy_full + s, (STATES_ONLY ? 2 : 4) * kTcPanel);
@@ -391,12 +393,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   } else if (warp == 18) {   // decays
     float raw[4], next[4];
     double total = 0.0;
-    if (count > 0) tc_load_logs(next, g, a.gs[1], chunk_of(0) * C, valid(chunk_of(0)), lane);
+    if (count > 0) tc_load_logs(next, g, a.gs[1], (int64_t)chunk_of(0) * C, valid(chunk_of(0)), lane);
 #pragma unroll 1
     for (int i = 0; i < count; ++i) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) raw[j] = next[j];
-      if (i + 1 < count) tc_load_logs(next, g, a.gs[1], chunk_of(i + 1) * C, valid(chunk_of(i + 1)), lane);
+      if (i + 1 < count) tc_load_logs(next, g, a.gs[1], (int64_t)chunk_of(i + 1) * C, valid(chunk_of(i + 1)), lane);
       if (i >= 2) wait_warp(lg_empty + (i & 1), ((i >> 1) - 1) & 1);
       tc_logs(Gs + (i & 1) * 2 * C, fac + (i & 1), raw, rev, lane, &total);
       arrive_warp(lg_full + (i & 1));
@@ -435,13 +437,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         if (part == 0) cs[row] = row_col;
       }
       const uint32_t pairs = rev ? ~0u << lane : ~0u >> (31 - lane);   // columns of the own block that count
+      const int64_t row_step = a.H * N, first_row = (b * a.T * a.H + h) * N + n0 + 32 * part;   // of the thread's columns
       // a chunk's rows to memory
       auto out = [&](int i, float win, float pair_sum) {
-        const int64_t t0 = chunk_of(i) * C, t = t0 + row;
-        const int n = valid(chunk_of(i)), sz = i & 1;
+        const int t = chunk_of(i) * C + row, n = valid(chunk_of(i)), sz = i & 1;
         const uint32_t at = lanes + (kLag ? (i & 1) * 64 : 0) + part * 32;
-        const int64_t first = ((b * a.T + t) * a.H + h) * N + n0;
-        const bool store = p.o && t < a.T;
+        const int64_t first = first_row + (int64_t)t * row_step;
+        const bool store = p.o && t < T;
         TcPair ext(0.f, 0.f);
         const TcPair win2(win, win), scale2(scale_in, scale_in);
         uint32_t vi[2][16], vo[2][16];
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             TcPair r[4];
-            const int piece = 2 * (2 * part + q) + e;
+            const int piece = 2 * (2 * part + q) + e, col = q * 16 + e * 8;   // of a row of Z; of the thread's columns
 #pragma unroll
             for (int j = 0; j < 4; ++j) r[j] = tc_pair(vi[q][e * 8 + 2 * j], vi[q][e * 8 + 2 * j + 1]) * win2;
             if (DOTS) {
@@ -469,18 +471,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
 #pragma unroll
             for (int j = 0; j < 4; ++j) r[j] = fma2(tc_pair(vo[q][e * 8 + 2 * j], vo[q][e * 8 + 2 * j + 1]), scale2, r[j]);
             if (store && n0 + piece * 8 < N) {
-              if (p.wide) {
+              if (WIDE) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                   const float2 v0 = r[2 * j].get(), v1 = r[2 * j + 1].get();
                   float4 v = make_float4(v0.x, v0.y, v1.x, v1.y);
                   if (row >= n) v = make_float4(0.f, 0.f, 0.f, 0.f);
-                  *reinterpret_cast<float4*>(static_cast<float*>(p.o) + first + piece * 8 + j * 4) = v;
+                  *reinterpret_cast<float4*>(static_cast<float*>(p.o) + first + col + j * 4) = v;
                 }
               } else {
                 uint4 pk = make_uint4(tc_pack(r[0]), tc_pack(r[1]), tc_pack(r[2]), tc_pack(r[3]));
                 if (row >= n) pk = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + first + piece * 8) = pk;
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + first + col) = pk;
               }
             }
           }
@@ -576,9 +578,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
       }
       // behind the sequence: zeros
       if (p.o) {
-        const int64_t first = max(c0, (len + C - 1) / C) * C, stop = min(a.T, c1 * C);
+        const int64_t first = (int64_t)(c0 + count) * C, stop = min(a.T, (int64_t)c1 * C);
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        const int pieces = min(8, (N - n0) / 8) * (p.wide ? 2 : 1), per = p.wide ? 4 : 8;
+        const int pieces = min(8, (N - n0) / 8) * (WIDE ? 2 : 1), per = WIDE ? 4 : 8;
         for (int64_t t = first + tid; t < stop; t += kTcRows)
           for (int q = 0; q < pieces; ++q) {
             const int64_t at = ((b * a.T + t) * a.H + h) * N + n0 + q * per;
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     };
 #pragma unroll 1
     for (int i = 0; i < count; ++i) {
-      const int64_t c = chunk_of(i);
+      const int c = chunk_of(i);
       const int n = valid(c), sz = i & 1, s = i % sxy;
       if (i > 0) advance(i - 1);
       dec = dec_now;
