@@ -499,8 +499,8 @@ int ptb_modal_bank_bwd(int dtype, int64_t rows, int64_t M, int64_t N, const void
  * dtype: PTB_F32, PTB_F64, PTB_F16 or PTB_BF16 for q, k, v, o and their gradients; log_decay, the states and their
  * gradients hold float64 beside PTB_F64, else float32.  q, k: (B,T,H,Dk), v: (B,T,H,Dv), 1 <= Dk, Dv <= 128, the last
  * axis dense; *_strides: three element strides (batch, time, head), zero where an axis is shared.  log_decay likewise
- * (batch and time stride zero: one decay per head); -inf is a decay of zero.  lengths: optional (B,), clamped to
- * 0..T: tokens from lengths[b] on are not read, leave the state alone and give zeros.  init, fin: optional dense
+ * (batch and time stride zero: one decay per head); -inf is a decay of zero.  lengths: optional (B,) of
+ * int32, or int64 when lengths_wide, clamped to 0..T: tokens from lengths[b] on are not read, leave the state alone and give zeros.  init, fin: optional dense
  * (B,H,Dk,Dv), the state before the first and after the last token.  o: dense (B,T,H,Dv), float32 when o_wide.
  * workspace: ptb_linear_attention_workspace_bytes(..., backward, decay_grad) bytes, 256-byte aligned, private to the
  * call until it completes; none (NULL) where that is 0.  status: as above (waits inside a CTA are bounded). */
@@ -509,7 +509,7 @@ int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, in
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const int32_t* lengths, const void* init, double scale, void* o, int o_wide, void* fin,
+                             const void* lengths, int lengths_wide, const void* init, double scale, void* o, int o_wide, void* fin,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream);
 /* Adjoint: the gradients of q, k, v (dense, shaped like them), of the log decays ((B,T,H) when
  * grad_log_decay_per_token, else (H)) and of the initial state, each optional.  grad_fin: optional gradient of fin.
@@ -517,7 +517,7 @@ int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t
 int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const int32_t* lengths, const void* init, double scale, const void* grad_o,
+                             const void* lengths, int lengths_wide, const void* init, double scale, const void* grad_o,
                              const int64_t* grad_o_strides, const void* grad_fin, void* grad_q, void* grad_k,
                              void* grad_v, void* grad_log_decay, int grad_log_decay_per_token, void* grad_init,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream);

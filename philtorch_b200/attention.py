@@ -96,7 +96,6 @@ def _check(q: Tensor, k: Tensor, v: Tensor, g: Tensor, init: Optional[Tensor], l
     if lengths is not None:
         torch._check(tuple(lengths.shape) == (B,), lambda: f"lengths must be ({B},), got {tuple(lengths.shape)}")
         torch._check(lengths.dtype in (torch.int32, torch.int64), lambda: f"lengths must be int32 or int64, got {lengths.dtype}")
-        torch._check(T < 2 ** 31, lambda: "lengths are for fewer than 2^31 tokens")
 
 
 def _decay_strides(g: Tensor):
@@ -116,12 +115,8 @@ def _workspace_bytes(code: int, B: int, T: int, H: int, Dk: int, Dv: int, backwa
     return n
 
 
-def _int_lengths(lengths: Optional[Tensor], T: int) -> Optional[Tensor]:
-    if lengths is None:
-        return None
-    if lengths.dtype == torch.int64:
-        lengths = lengths.clamp(0, T).to(torch.int32)
-    return lengths.contiguous()
+def _lengths_args(lengths: Optional[Tensor]):
+    return (None, 0) if lengths is None else (lengths.data_ptr(), int(lengths.dtype == torch.int64))
 
 
 # ------------------------------------------------------------------------------------------------ ops
@@ -142,12 +137,12 @@ def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state, wide
     Dv = v.shape[3]
     q, k, v = _rows(q), _rows(k), _rows(v)
     init = None if init is None else init.contiguous()
-    lengths = _int_lengths(lengths, T)
+    lengths = None if lengths is None else lengths.contiguous()
     o = (log_decay if wide else v).new_empty((B, T, H, Dv))   # wide: in the sums' type, for a normalisation that follows
     state = log_decay.new_empty((B, H, Dk, Dv) if want_state else (0,))
     if B and H and (T or want_state):
         _lib.call(lib.ptb_linear_attention_fwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k), _outer_strides(k),
-                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(o),
+                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), *_lengths_args(lengths), ptr(init), scale, ptr(o),
                   int(o.dtype != v.dtype), ptr(state) if want_state else None, ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 0, 0))
     return o, state
 
@@ -163,14 +158,14 @@ def _linear_attention_bwd(q, k, v, log_decay, init, lengths, scale, grad_o, grad
     q, k, v, grad_o = _rows(q), _rows(k), _rows(v), _rows(grad_o)
     init = None if init is None else init.contiguous()
     grad_state = None if grad_state is None else grad_state.contiguous()
-    lengths = _int_lengths(lengths, T)
+    lengths = None if lengths is None else lengths.contiguous()
     gq, gk, gv = (t.new_empty(t.shape if need else (0,)) for t, need in ((q, need_q), (k, need_k), (v, need_v)))
     gg = log_decay.new_empty(log_decay.shape if need_decay else (0,))
     ginit = log_decay.new_empty((B, H, Dk, Dv) if need_init else (0,))
     if B and H:
         opt = lambda t, need: ptr(t) if need else None   # noqa: E731
         _lib.call(lib.ptb_linear_attention_bwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k), _outer_strides(k),
-                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), ptr(lengths), ptr(init), scale, ptr(grad_o),
+                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), *_lengths_args(lengths), ptr(init), scale, ptr(grad_o),
                   _outer_strides(grad_o), ptr(grad_state), opt(gq, need_q), opt(gk, need_k), opt(gv, need_v),
                   opt(gg, need_decay), int(log_decay.dim() == 3), opt(ginit, need_init),
                   ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 1, int(need_decay)))

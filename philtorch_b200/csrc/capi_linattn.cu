@@ -336,7 +336,7 @@ static void la_strides(int64_t (&d)[3], const int64_t* s) { for (int i = 0; i < 
 template <class T, class S>
 static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs,
                   const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
-                  const int64_t* gs, const int32_t* lengths, const void* init, double scale, void* o, int o_wide, void* fin,
+                  const int64_t* gs, LaLengths lengths, const void* init, double scale, void* o, int o_wide, void* fin,
                   void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
   LaArgs<S> a = {};
   LaPass<S>& p = a.p[0];
@@ -362,7 +362,7 @@ static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
 template <class T, class S>
 static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs,
                   const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
-                  const int64_t* gs, const int32_t* lengths, const void* init, double scale, const void* go,
+                  const int64_t* gs, LaLengths lengths, const void* init, double scale, const void* go,
                   const int64_t* gos, const void* gfin, void* gq, void* gk, void* gv, void* gg, int gg_per_token,
                   void* ginit, void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
   const bool dec = gg != nullptr;
@@ -498,19 +498,19 @@ int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, in
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const int32_t* lengths, const void* init, double scale, void* o, int o_wide, void* fin,
+                             const void* lengths, int lengths_wide, const void* init, double scale, void* o, int o_wide, void* fin,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
   if (int rc = la_check(dtype, B, T, H, Dk, Dv)) return rc;
   if (B == 0 || H == 0) return PTB_OK;
   if ((T > 0 && (!q || !k || !v || !o || !log_decay)) || !q_strides || !k_strides || !v_strides || !log_decay_strides) return PTB_ERR_ARG;
   PTB_LA_TYPES((la_fwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
-                               lengths, init, scale, o, o_wide, fin, workspace, workspace_bytes, status, (cudaStream_t)stream)))
+                               LaLengths{lengths, lengths_wide}, init, scale, o, o_wide, fin, workspace, workspace_bytes, status, (cudaStream_t)stream)))
 }
 
 int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const int32_t* lengths, const void* init, double scale, const void* grad_o,
+                             const void* lengths, int lengths_wide, const void* init, double scale, const void* grad_o,
                              const int64_t* grad_o_strides, const void* grad_fin, void* grad_q, void* grad_k,
                              void* grad_v, void* grad_log_decay, int grad_log_decay_per_token, void* grad_init,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
@@ -520,7 +520,7 @@ int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t
       !grad_o_strides)
     return PTB_ERR_ARG;
   PTB_LA_TYPES((la_bwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
-                               lengths, init, scale, grad_o, grad_o_strides, grad_fin, grad_q, grad_k, grad_v,
+                               LaLengths{lengths, lengths_wide}, init, scale, grad_o, grad_o_strides, grad_fin, grad_q, grad_k, grad_v,
                                grad_log_decay, grad_log_decay_per_token, grad_init, workspace, workspace_bytes,
                                status, (cudaStream_t)stream)))
 }

@@ -23,6 +23,11 @@ namespace ptb {
 constexpr int kLaMaxDim = 128;       // largest Dk and Dv
 constexpr double kLaMinLog = -1e5;   // stands for a decay of zero (exp of it is 0 in double)
 
+struct LaLengths {
+  const void* p;   // may be NULL: every sequence has T tokens
+  int wide;        // int64, else int32
+};
+
 // one pass; x: (B,T,H,M), y: (B,T,H,M), z: (B,T,H,N), o: dense (B,T,H,N); strides in elements (b, t, h)
 template <class S>
 struct LaPass {
@@ -44,7 +49,7 @@ struct LaArgs {
   LaPass<S> p[3];
   const S* g;
   int64_t gs[3];
-  const int32_t* lengths;   // may be NULL; per b, clamped to 0..T
+  LaLengths lengths;        // per b, clamped to 0..T
   int64_t B, T, H;
   int nseg, seg_chunks;     // the time axis is cut into nseg segments of seg_chunks chunks
   S* seg;                   // [role][segment][bh][M*N] entering states of segments (first in pass order unused)
@@ -62,9 +67,9 @@ template <class T, class S> __device__ __forceinline__ void la_store(T* p, S v) 
 template <> __device__ __forceinline__ void la_store<__half, float>(__half* p, float v) { *p = __float2half_rn(v); }
 template <> __device__ __forceinline__ void la_store<__nv_bfloat16, float>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ int64_t la_length(const int32_t* lengths, int64_t b, int64_t T) {
-  if (!lengths) return T;
-  const int64_t n = lengths[b];
+__device__ __forceinline__ int64_t la_length(const LaLengths& lengths, int64_t b, int64_t T) {
+  if (!lengths.p) return T;
+  const int64_t n = lengths.wide ? static_cast<const int64_t*>(lengths.p)[b] : static_cast<const int32_t*>(lengths.p)[b];
   return n < 0 ? 0 : (n > T ? T : n);
 }
 
@@ -443,7 +448,7 @@ struct LaDecayArgs {
   int q_slices, k_slices;
   const S* g;
   int64_t gs[3];
-  const int32_t* lengths;
+  LaLengths lengths;
   int64_t B, T, H, MN, used;      // scalars between two states, and how many of them count
   S* dg;           // (B,T,H), or NULL
   double* part;    // [chunk][bh] sums over a chunk, or NULL

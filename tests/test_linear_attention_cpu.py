@@ -56,7 +56,7 @@ def test_c_entry_points_refuse():
     s = I3(8, 8, 8)
 
     def fwd(dtype=0, B=1, T=4, H=1, Dk=8, Dv=8, q=p, ws=None, wsb=0):
-        return lib.ptb_linear_attention_fwd(dtype, B, T, H, Dk, Dv, q, s, p, s, p, s, p, s, None, None, 1.0, p, 0, None, ws, wsb,
+        return lib.ptb_linear_attention_fwd(dtype, B, T, H, Dk, Dv, q, s, p, s, p, s, p, s, None, 0, None, 1.0, p, 0, None, ws, wsb,
                                             None, None)
 
     assert fwd(dtype=2) == 1 and fwd(dtype=9) == 1          # no complex numbers
