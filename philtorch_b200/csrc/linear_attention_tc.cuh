@@ -4,16 +4,28 @@
 // A CTA walks one (b, h, segment) in chunks of 128 tokens with a slice of 64 columns of the state.  Four products per
 // chunk, issued by one thread:
 //   SC = X Y^T (128 x 128)         OI = X S (128 x 64)        O = P Z (P from tensor memory)        U = Y^T Zw
-// around which two groups of four warps work, one thread per row:
-//   rows   P = SC * decays, rounded to bfloat16, back into tensor memory; then o = po (O + win OI) to memory
-//   state  S <- exp(E) S + U in registers (float32, one row of the state per thread); S and the weighted Zw go to shared
-//          memory as bfloat16 operands
-// and single threads drive the TMA loads (X and Y double-buffered, no multicast) and the products.  U of a chunk does
-// not wait for the state, so the chain from chunk to chunk is one multiply-add per element of the state.
+// around which two groups of eight warps work, two threads per row:
+//   rows   P = SC * decays, rounded to bfloat16, back into tensor memory; then o = po (pz O + win OI) to memory, a chunk
+//          later: while the next chunk's products run
+//   state  S <- exp(E) S + U in registers (float32); S and the weighted Zw go to shared memory as bfloat16 operands
+// and single warps drive the TMA loads (no multicast), the products and the running sums of the decays.  U of a
+// chunk does not wait for the state, so the chain from chunk to chunk is one multiply-add per element of the state.
 //
 // Accuracy as in linear_attention_mma.cuh: one rounding of P and of S to bfloat16 where the result is bfloat16; Zw in
-// two terms, three for a float32 final state; with `dots` (gradient of the decays) S and Zw in three terms, and the
+// two terms, three for a float32 final state; with DOTS (gradient of the decays) S and Zw in three terms, and the
 // pairs inside a chunk from the float32 scores themselves.
+//
+// Why this shape.  128 rows fill the tensor core; 64 columns leave room in shared memory (227 KB) for two stages of
+// X, Y and Z beside three terms of Zw, and in tensor memory for a second O and OI; the price is that both slices of
+// a head form the scores.  Eight warps a group instead of four: 238 -> 203 us (B=4, T=8192, H=16, D=128, final state).
+// Loops instead of straight-line code wherever the tensor-memory tiles allow it: unrolled, the warps' different roles
+// did not fit the instruction cache together, and the kernel ran at the rate of the instruction fetch (718 -> 337 us).
+// Rows leaving a chunk later: 203 -> 178 us.  Tried and dropped: P in the place of the scores with U in one
+// product (194 us: the next scores then wait for O), loading the next scores ahead in registers (216 us),
+// prefetching tiles into L2 (no change), 32-byte stores (2.3 -> 3.1 us a chunk).
+// What bounds it: 2.3 us a chunk and CTA, in which the row group (weights 1.0, output 0.6 us) and the issue order
+// of the products alternate; tensor pipe 33 % busy, DRAM 29 %; with 128 SMs busy the 1000 W limit holds the clock at
+// 1.6 GHz.  183 us without the final state, 201 us with it (537 MB: floor 82 us).
 #pragma once
 #include "linear_attention_mma.cuh"
 #include "packed.cuh"

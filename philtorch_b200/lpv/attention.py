@@ -30,6 +30,10 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Opt
         norm_eps, norm_weight, norm_bias: with norm_eps, the output of each head is normalised by
             ``layer_norm`` (one group of Dv channels per head; weight and bias (H * Dv,)).
 
+    bfloat16 tensors of more than 32 tokens run on the tensor cores: weights and states are rounded to bfloat16
+    once where they enter a product (sums, states and the decays' gradient are float32), and an infinite or NaN
+    value reaches the outputs of up to 127 tokens before it.
+
     Returns:
         o (B, T, H, Dv), or (o, state).  Differentiable once in q, k, v, log_decay, zi (and the norm's
         parameters).
