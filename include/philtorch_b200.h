@@ -500,16 +500,20 @@ int ptb_modal_bank_bwd(int dtype, int64_t rows, int64_t M, int64_t N, const void
  * gradients hold float64 beside PTB_F64, else float32.  q, k: (B,T,H,Dk), v: (B,T,H,Dv), 1 <= Dk, Dv <= 128, the last
  * axis dense; *_strides: three element strides (batch, time, head), zero where an axis is shared.  log_decay likewise
  * (batch and time stride zero: one decay per head); -inf is a decay of zero.  lengths: optional (B,) of
- * int32, or int64 when lengths_wide, clamped to 0..T: tokens from lengths[b] on are not read, leave the state alone and give zeros.  init, fin: optional dense
+ * int32, or int64 when lengths_wide, clamped to 0..T:
+ * tokens from lengths[b] on are not read, leave the state alone and give zeros.  init, fin: optional dense
  * (B,H,Dk,Dv), the state before the first and after the last token.  o: dense (B,T,H,Dv), float32 when o_wide.
- * workspace: ptb_linear_attention_workspace_bytes(..., backward, decay_grad) bytes, 256-byte aligned, private to the
+ * copies: PTB_BF16 and T > 32 only (else ignored): bit 0, 1, 2, 3 for q, k, v, grad_o.  Their rows have to start on
+ * 16 bytes (base pointer 16-byte aligned; strides of axes longer than one a multiple of 8 elements, and not zero in
+ * time); a marked operand need not, it is copied to the workspace first.  Unmarked and unaligned: PTB_ERR_ARG.
+ * workspace: ptb_linear_attention_workspace_bytes(..., backward, decay_grad, copies) bytes, 256-byte aligned, private to the
  * call until it completes; none (NULL) where that is 0.  status: as above (waits inside a CTA are bounded). */
 int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
-                                             int backward, int decay_grad);
+                                             int backward, int decay_grad, int copies);
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const void* lengths, int lengths_wide, const void* init, double scale, void* o, int o_wide, void* fin,
+                             const void* lengths, int lengths_wide, const void* init, double scale, int copies, void* o, int o_wide, void* fin,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream);
 /* Adjoint: the gradients of q, k, v (dense, shaped like them), of the log decays ((B,T,H) when
  * grad_log_decay_per_token, else (H)) and of the initial state, each optional.  grad_fin: optional gradient of fin.
@@ -517,7 +521,7 @@ int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t
 int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const void* lengths, int lengths_wide, const void* init, double scale, const void* grad_o,
+                             const void* lengths, int lengths_wide, const void* init, double scale, int copies, const void* grad_o,
                              const int64_t* grad_o_strides, const void* grad_fin, void* grad_q, void* grad_k,
                              void* grad_v, void* grad_log_decay, int grad_log_decay_per_token, void* grad_init,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream);

@@ -105,14 +105,25 @@ def _decay_strides(g: Tensor):
 _ws_bytes: dict = {}
 
 
-def _workspace_bytes(code: int, B: int, T: int, H: int, Dk: int, Dv: int, backward: int, decay: int) -> int:
-    key = (code, B, T, H, Dk, Dv, backward, decay)
+def _workspace_bytes(*key) -> int:
     n = _ws_bytes.get(key)
     if n is None:
         if len(_ws_bytes) > 4096:   # a server sees many lengths
             _ws_bytes.clear()
-        n = _ws_bytes[key] = lib.ptb_linear_attention_workspace_bytes(code, B, T, H, Dk, Dv, backward, decay)
+        n = _ws_bytes[key] = lib.ptb_linear_attention_workspace_bytes(*key)
     return n
+
+
+def _copies(T: int, *tensors: Tensor) -> int:
+    """The operands whose rows the tensor-core kernels' TMA loads cannot address, a bit for each: they are copied."""
+    if T <= 32 or tensors[0].dtype != torch.bfloat16:
+        return 0
+    mask = 0
+    for i, t in enumerate(tensors):
+        b, s, h, _ = t.stride()
+        if t.data_ptr() % 16 or s % 8 or s == 0 or (h % 8 and t.shape[2] > 1) or (b % 8 and t.shape[0] > 1):
+            mask |= 1 << i
+    return mask
 
 
 def _lengths_args(lengths: Optional[Tensor]):
@@ -141,9 +152,11 @@ def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state, wide
     o = (log_decay if wide else v).new_empty((B, T, H, Dv))   # wide: in the sums' type, for a normalisation that follows
     state = log_decay.new_empty((B, H, Dk, Dv) if want_state else (0,))
     if B and H and (T or want_state):
+        copies = _copies(T, q, k, v)
         _lib.call(lib.ptb_linear_attention_fwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k), _outer_strides(k),
-                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), *_lengths_args(lengths), ptr(init), scale, ptr(o),
-                  int(o.dtype != v.dtype), ptr(state) if want_state else None, ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 0, 0))
+                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), *_lengths_args(lengths), ptr(init), scale, copies,
+                  ptr(o),
+                  int(o.dtype != v.dtype), ptr(state) if want_state else None, ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 0, 0, copies))
     return o, state
 
 
@@ -163,12 +176,14 @@ def _linear_attention_bwd(q, k, v, log_decay, init, lengths, scale, grad_o, grad
     gg = log_decay.new_empty(log_decay.shape if need_decay else (0,))
     ginit = log_decay.new_empty((B, H, Dk, Dv) if need_init else (0,))
     if B and H:
+        copies = _copies(T, q, k, v, grad_o)
         opt = lambda t, need: ptr(t) if need else None   # noqa: E731
         _lib.call(lib.ptb_linear_attention_bwd, dev, B, T, code, B, T, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k), _outer_strides(k),
-                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), *_lengths_args(lengths), ptr(init), scale, ptr(grad_o),
+                  ptr(v), _outer_strides(v), ptr(log_decay), _decay_strides(log_decay), *_lengths_args(lengths), ptr(init), scale, copies,
+                  ptr(grad_o),
                   _outer_strides(grad_o), ptr(grad_state), opt(gq, need_q), opt(gk, need_k), opt(gv, need_v),
                   opt(gg, need_decay), int(log_decay.dim() == 3), opt(ginit, need_init),
-                  ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 1, int(need_decay)))
+                  ws_bytes=_workspace_bytes(code, B, T, H, Dk, Dv, 1, int(need_decay), copies))
     else:
         gg.zero_()
     return gq, gk, gv, gg, ginit

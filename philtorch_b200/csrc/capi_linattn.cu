@@ -1,6 +1,5 @@
 // C ABI of linear attention with decays (see include/philtorch_b200.h).
 #include "linear_attention.cuh"
-#include "linear_attention_mma.cuh"
 #include "linear_attention_tc.cuh"
 
 namespace ptb {
@@ -14,7 +13,7 @@ constexpr int kLaSms = 148;   // CTAs to aim for; only the cut of the time axis 
 struct LaPlan {
   int C, slices_max, nseg, seg_chunks;
   int64_t nchunk, seg_off, log_off, qb_off, rb_off, qd_off, kd_off, part_off, total;
-  int64_t seg_stride, bound_elems;
+  int64_t seg_stride, bound_elems, copy_off[4], out_off[3];
 };
 
 // Few (batch, head) pairs: the time axis is cut into segments that run side by side.  Their entering states
@@ -35,7 +34,7 @@ struct LaSize { int64_t B, T, H, Dk, Dv; };
 // C: tokens of a chunk; width: columns of a state that a CTA takes; mn: scalars of a stored state
 template <class S>
 static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int width, int64_t mn, int per_sm, int slots) {
-  LaPlan l;
+  LaPlan l = {};
   l.C = C;
   const int64_t over_k = (z.Dk + width - 1) / width, over_v = (z.Dv + width - 1) / width;
   l.slices_max = (int)std::max(over_k, over_v);
@@ -62,23 +61,36 @@ static LaPlan la_simt_plan(const LaSize& z, int roles, bool decay_grad) {
   using G = LaGeom<S>;
   return la_plan<S>(z, roles, decay_grad, G::C, G::NS, z.Dk * z.Dv, G::PER_SM, 0);
 }
-// the tensor-core kernels come for head sizes up to 64 and up to 128
-static int la_mma_width(const LaSize& z) { return std::max(z.Dk, z.Dv) <= 64 ? 64 : 128; }
-static LaPlan la_mma_plan(const LaSize& z, int roles, bool decay_grad) {
-  const int64_t W = la_mma_width(z);
-  return la_plan<float>(z, roles, decay_grad, kLaMmaChunk, kLaMaxDim, W * W, W == 64 ? 4 : 2, 1);
-}
-static LaPlan la_tc_plan(const LaSize& z, int roles, bool decay_grad) {
-  return la_plan<float>(z, roles, decay_grad, kTcChunk, kTcSlice, kTcDim * kTcDim, 1, 1);
-}
-enum LaPath { kLaSimt, kLaMma, kLaTc };
-template <class S>
-static LaPlan la_plan_of(LaPath path, const LaSize& z, int roles, bool decay_grad) {
-  if constexpr (std::is_same<S, float>::value) {
-    if (path == kLaMma) return la_mma_plan(z, roles, decay_grad);
-    if (path == kLaTc) return la_tc_plan(z, roles, decay_grad);
+static LaPlan la_tc_plan(const LaSize& z, int roles, bool decay_grad, int copies) {
+  LaPlan l = la_plan<float>(z, roles, decay_grad, kTcChunk, kTcSlice, kTcDim * kTcDim, 1, 1);
+  auto take = [&](int64_t D, int size) {
+    const int64_t o = l.total;
+    l.total += align_up(z.B * z.T * z.H * align_up(D, 8) * size, 256);
+    return o;
+  };
+  for (int k = 0; k < 4; ++k)   // q, k, v, grad_o on rows that start on 16 bytes
+    if (copies >> k & 1) l.copy_off[k] = take(k < 2 ? z.Dk : z.Dv, 2);
+  if (roles == 1) {
+    if (z.Dv % 8) l.out_off[0] = take(z.Dv, 4);   // o, which may be float32
+  } else {
+    for (int r = 0; r < 3; ++r)   // dq, dk, dv
+      if ((r < 2 ? z.Dk : z.Dv) % 8) l.out_off[r] = take(r < 2 ? z.Dk : z.Dv, 2);
   }
+  return l;
+}
+template <class S>
+static LaPlan la_plan_of(bool tensor_cores, const LaSize& z, int roles, bool decay_grad, int copies) {
+  if constexpr (std::is_same<S, float>::value)
+    if (tensor_cores) return la_tc_plan(z, roles, decay_grad, copies);
   return la_simt_plan<S>(z, roles, decay_grad);
+}
+
+// bfloat16 runs on the tensor cores but for one chunk of the CUDA-core kernels: as fast there (B=1, H=4, D=64, T=1: 9.2
+// against 11.4 us; T=64: 16.1 against 10.3), and where an output is a sum of a few terms, the rounding of their
+// weights to bfloat16 would not average out.
+template <class T>
+static bool la_tensor_cores(int64_t tokens) {
+  return std::is_same<T, __nv_bfloat16>::value && tokens > LaGeom<float>::C;
 }
 
 template <class T, class S, int MD, bool STATES_ONLY>
@@ -125,95 +137,109 @@ static int la_simt_run(LaArgs<S>& a, int roles, cudaStream_t st) {
   return la_simt_launch<T, S, MD, false>(a, roles, st);
 }
 
-template <int W, bool VEC, bool STATES_ONLY>
-static int la_mma_launch(const LaArgs<float>& a, const LaMmaFlags& f, int roles, bool dots, cudaStream_t st) {
-  static bool ready[kMaxDevices] = {};
-  int dev = 0;
-  PTB_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= kMaxDevices) return PTB_ERR_ARG;
-  const int smem = LaMmaSmem<W, W>::bytes(f.stages, dots);
-  {
-    std::lock_guard<std::mutex> lock(init_mutex());
-    if (!ready[dev]) {
-      PTB_CUDA(cudaFuncSetAttribute(la_mma_kernel<W, W, VEC, STATES_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    LaMmaSmem<W, W>::bytes(2, false)));   // the most that is ever asked for
-      ready[dev] = true;
-    }
+// ---- tcgen05 kernels
+// (Dv | Dk, T, H, B) view of an operand, box 64 x 128 tokens; an axis of stride zero (or of one entry) is left out
+static int la_tc_map(LaTcMap* m, const void* base, const int64_t* st, int64_t B, int64_t T, int64_t H, int64_t D) {
+  const EncodeTiledFn enc = tensor_map_encoder();
+  if (!enc) return PTB_ERR_CUDA;
+  m->bmul = B > 1 && st[0] != 0;
+  m->hmul = H > 1 && st[2] != 0;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)(m->hmul ? H : 1), (cuuint64_t)(m->bmul ? B : 1)};
+  const cuuint64_t strides[3] = {(cuuint64_t)st[1] * 2, (cuuint64_t)(m->hmul ? st[2] * 2 : 16), (cuuint64_t)(m->bmul ? st[0] * 2 : 16)};
+  if (!aligned16(base) || st[1] == 0) return PTB_ERR_ARG;
+  for (cuuint64_t v : strides)
+    if (v % 16 || v >= (1ull << 40)) return PTB_ERR_ARG;
+  const cuuint32_t box[4] = {64u, (cuuint32_t)kTcChunk, 1u, 1u}, estr[4] = {1u, 1u, 1u, 1u};
+  return enc(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? PTB_OK : PTB_ERR_ARG;
+}
+
+static int la_tc_setup(LaTcArgs* k, const LaArgs<float>& a, int roles) {
+  for (int r = 0; r < roles; ++r) {
+    const LaPass<float>& p = a.p[r];
+    if (!aligned16(p.o)) return PTB_ERR_ARG;   // written in pieces of 16 bytes
+    if (int rc = la_tc_map(&k->x[r], p.x, p.xs, a.B, a.T, a.H, p.M)) return rc;
+    if (int rc = la_tc_map(&k->y[r], p.y, p.ys, a.B, a.T, a.H, p.M)) return rc;
+    if (int rc = la_tc_map(&k->z[r], p.z, p.zs, a.B, a.T, a.H, p.N)) return rc;
+    if (p.w)
+      if (int rc = la_tc_map(&k->w[r], p.w, p.ws, a.B, a.T, a.H, p.N)) return rc;
   }
-  const int64_t grid = a.B * a.H * (STATES_ONLY ? a.nseg - (f.all_segments ? 0 : 1) : a.nseg);
-  if (grid > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
-  la_mma_kernel<W, W, VEC, STATES_ONLY><<<dim3((unsigned)grid, roles), 128, smem, st>>>(a, f);
+  return PTB_OK;
+}
+
+// n arrays of rows, moved in one launch
+static int la_move(LaMoveArgs& m, int n, const LaSize& z, cudaStream_t st) {
+  if (n == 0) return PTB_OK;
+  m.T = z.T;
+  m.H = z.H;
+  m.rows = z.B * z.T * z.H;
+  uint64_t bits = 16;
+  for (int i = 0; i < n; ++i) {
+    bits |= reinterpret_cast<uintptr_t>(m.src[i]) | reinterpret_cast<uintptr_t>(m.dst[i]) | m.width[i] | m.pitch[i] | m.st[i][1];
+    if (z.B > 1) bits |= m.st[i][0];
+    if (z.H > 1) bits |= m.st[i][2];
+  }
+  const int64_t ctas = (m.rows + kLaMoveRows - 1) / kLaMoveRows;
+  if (ctas > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)ctas, n);
+  switch (bits & (~bits + 1)) {   // the largest power of two that divides all of them
+    case 16: la_move_kernel<uint4><<<grid, 256, 0, st>>>(m); break;
+    case 8: la_move_kernel<uint2><<<grid, 256, 0, st>>>(m); break;
+    case 4: la_move_kernel<uint32_t><<<grid, 256, 0, st>>>(m); break;
+    default: la_move_kernel<uint16_t><<<grid, 256, 0, st>>>(m); break;
+  }
   PTB_CUDA(cudaGetLastError());
   return PTB_OK;
 }
 
-template <int W, bool VEC>
-static int la_mma_run(const LaArgs<float>& a, int roles, bool dots, cudaStream_t st) {
-  LaMmaFlags main = {}, states = {};
-  // one buffer of the operands beside w, else two: either way two CTAs fit an SM
-  main.stages = dots ? 1 : 2;
-  states.stages = 2;
-  for (int r = 0; r < roles; ++r) {
-    // with dots, the states kept at the chunks' ends and what is read from them are float32 results; otherwise
-    // only the final state is one, and where the row is cut, the pass that forms the segments' states gives it
-    const bool exact = a.p[r].dots, end = a.p[r].fin && !exact;
-    main.accurate[r] = exact ? 3 : end && a.nseg == 1 ? 1 : 0;
-    states.accurate[r] = exact || end ? 1 : 0;
-    if (end && a.nseg > 1) main.all_segments = states.all_segments = 1;
+// q, k, v, grad_o of a call; those marked in `copies` move to the workspace, on rows that start on 16 bytes
+struct LaOperands {
+  const void* p[4];
+  int64_t st[4][3];
+};
+static int la_copy_in(LaOperands* o, int copies, const LaSize& z, const LaPlan& l, void* ws, cudaStream_t st) {
+  LaMoveArgs m = {};
+  int n = 0;
+  for (int k = 0; k < 4; ++k) {
+    if (!(copies >> k & 1) || !o->p[k]) continue;
+    const int64_t D = k < 2 ? z.Dk : z.Dv, P = align_up(D, 8);
+    m.src[n] = static_cast<const char*>(o->p[k]);
+    m.dst[n] = static_cast<char*>(ws) + l.copy_off[k];
+    for (int i = 0; i < 3; ++i) m.st[n][i] = o->st[k][i] * 2;
+    m.width[n] = (int)D * 2;
+    m.pitch[n] = P * 2;
+    o->p[k] = m.dst[n++];
+    o->st[k][0] = z.T * z.H * P;
+    o->st[k][1] = z.H * P;
+    o->st[k][2] = P;
   }
-  if (a.nseg > 1) {
-    if (int rc = la_mma_launch<W, VEC, true>(a, states, roles, false, st)) return rc;
-    const int64_t elems = a.B * a.H * W * W;
-    if (elems / 256 > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
-    la_mma_join_kernel<W, W><<<dim3((unsigned)((elems + 255) / 256), roles), 256, 0, st>>>(a, states);
-    PTB_CUDA(cudaGetLastError());
-  }
-  return la_mma_launch<W, VEC, false>(a, main, roles, dots, st);
+  return la_move(m, n, z, st);
 }
 
-// 16-byte accesses: every operand's rows start on 16 bytes and hold a multiple of 8 values
-static bool la_mma_vec(const LaArgs<float>& a, int roles) {
+// The rows of results whose head size is no multiple of eight are written to the workspace, as whole 16-byte pieces,
+// and moved from there: written in place, element by element, they cost four times the kernel's own time (B=4, T=2048,
+// H=16, D=60: 202 against 44 us).
+template <class S>
+static LaMoveArgs la_results(LaArgs<S>& a, int roles, const LaPlan& l, void* ws, int* n) {
+  LaMoveArgs m = {};
+  *n = 0;
   for (int r = 0; r < roles; ++r) {
-    const LaPass<float>& p = a.p[r];
-    if (p.M % 8 || p.N % 8 || !aligned16(p.x) || !aligned16(p.y) || !aligned16(p.z) || !aligned16(p.w) || !aligned16(p.o)) return false;
-    for (int i = 0; i < 3; ++i)
-      if (p.xs[i] % 8 || p.ys[i] % 8 || p.zs[i] % 8 || p.ws[i] % 8) return false;
+    LaPass<S>& p = a.p[r];
+    p.pitch = (int)align_up(p.N, 8);
+    if (!p.o || p.pitch == p.N) continue;
+    const int64_t size = p.wide ? 4 : 2, P = p.pitch * size;
+    m.dst[*n] = static_cast<char*>(p.o);
+    p.o = static_cast<char*>(ws) + l.out_off[p.out];
+    m.src[*n] = static_cast<const char*>(p.o);
+    m.st[*n][0] = a.T * a.H * P;
+    m.st[*n][1] = a.H * P;
+    m.st[*n][2] = P;
+    m.width[*n] = (int)(p.N * size);
+    m.pitch[*n] = p.N * size;
+    ++*n;
   }
-  return true;
-}
-
-// ---- tcgen05 kernels
-// (Dv | Dk, T, H, B) view of an operand, box 64 x 128 tokens; an axis of stride zero (or of one entry) is left out
-static bool la_tc_map(LaTcMap* m, const void* base, const int64_t* st, int64_t B, int64_t T, int64_t H, int64_t D) {
-  const EncodeTiledFn enc = tensor_map_encoder();
-  if (!enc || !base) return false;
-  m->bmul = B > 1 && st[0] != 0;
-  m->hmul = H > 1 && st[2] != 0;
-  const int64_t ts = T > 1 ? st[1] : D;
-  if (ts == 0 && T > 1) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)(m->hmul ? H : 1), (cuuint64_t)(m->bmul ? B : 1)};
-  const cuuint64_t strides[3] = {(cuuint64_t)(T > 1 ? ts * 2 : 16), (cuuint64_t)(m->hmul ? st[2] * 2 : 16),
-                                 (cuuint64_t)(m->bmul ? st[0] * 2 : 16)};
-  for (cuuint64_t v : strides)
-    if (v % 16 || v >= (1ull << 40)) return false;
-  const cuuint32_t box[4] = {64u, (cuuint32_t)kTcChunk, 1u, 1u}, estr[4] = {1u, 1u, 1u, 1u};
-  return enc(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// The tcgen05 kernels take every size whose operands the TMA unit can address; the mma.sync kernels the others
-// (odd or unaligned head sizes).  B=1, H=4, D=64, T=256: 31.6 us on mma.sync, 11.4 us here.
-static bool la_tc_setup(LaTcArgs* k, const LaArgs<float>& a, int roles) {
-  if (a.T < 1 || a.T > 0x7fffffffll || !la_mma_vec(a, roles)) return false;
-  for (int r = 0; r < roles; ++r) {
-    const LaPass<float>& p = a.p[r];
-    if (!la_tc_map(&k->x[r], p.x, p.xs, a.B, a.T, a.H, p.M) || !la_tc_map(&k->y[r], p.y, p.ys, a.B, a.T, a.H, p.M) ||
-        !la_tc_map(&k->z[r], p.z, p.zs, a.B, a.T, a.H, p.N))
-      return false;
-    if (p.w && !la_tc_map(&k->w[r], p.w, p.ws, a.B, a.T, a.H, p.N)) return false;
-  }
-  return true;
+  return m;
 }
 
 // beside: may start while the kernel launched before it on the stream is running (it reads nothing that one writes)
@@ -262,11 +288,9 @@ static int la_tc_run(LaTcArgs& k, int roles, cudaStream_t st) {
     k.xy_stages = 2;
     k.dots = 0;
     if (int rc = la_tc_launch<true, false>(k, roles, st)) return rc;
-    LaMmaFlags f = {};
-    f.all_segments = k.all_segments;
     const int64_t elems = a.B * a.H * kTcDim * kTcDim;
     if (elems / 256 > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
-    la_mma_join_kernel<kTcDim, kTcDim><<<dim3((unsigned)((elems + 255) / 256), roles), 256, 0, st>>>(a, f);
+    la_tc_join_kernel<<<dim3((unsigned)((elems + 255) / 256), roles), 256, 0, st>>>(a, k.all_segments);
     PTB_CUDA(cudaGetLastError());
     for (int r = 0; r < roles; ++r)   // the segments' states are known: the update needs no float32 end any more
       if (!a.p[r].dots) k.nu[r] = 2;
@@ -296,82 +320,72 @@ static int la_tc_run(LaTcArgs& k, int roles, cudaStream_t st) {
 }
 
 template <class T, class S>
-static int la_run(LaArgs<S>& a, LaTcArgs* k, LaPath path, int roles, const LaPlan& l, void* ws, uint32_t* status, cudaStream_t st) {
+static int la_run(LaArgs<S>& a, int roles, const LaPlan& l, void* ws, uint32_t* status, cudaStream_t st) {
   la_workspace(a, l, ws);
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    if (path == kLaTc) {
-      k->a = a;
-      k->status = status;
-      k->wait_cycles = (long long)(g_wait_ns * 2);   // SM clocks are below 2 GHz
-      return la_tc_run(*k, roles, st);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    if (la_tensor_cores<T>(a.T)) {
+      LaTcArgs k = {};
+      int moved;
+      LaMoveArgs m = la_results(a, roles, l, ws, &moved);
+      if (int rc = la_tc_setup(&k, a, roles)) return rc;
+      k.a = a;
+      k.status = status;
+      k.wait_cycles = (long long)(g_wait_ns * 2);   // SM clocks are below 2 GHz
+      if (int rc = la_tc_run(k, roles, st)) return rc;
+      return la_move(m, moved, LaSize{a.B, a.T, a.H, 0, 0}, st);
     }
-    bool dots = false;
-    for (int r = 0; r < roles; ++r) dots = dots || a.p[r].dots;
-    const bool vec = la_mma_vec(a, roles);
-    if (path == kLaMma) {
-      if (std::max(a.p[0].M, a.p[0].N) <= 64)
-        return vec ? la_mma_run<64, true>(a, roles, dots, st) : la_mma_run<64, false>(a, roles, dots, st);
-      return vec ? la_mma_run<128, true>(a, roles, dots, st) : la_mma_run<128, false>(a, roles, dots, st);
-    }
-  }
   int most = 0;   // channels of x and y
   for (int r = 0; r < roles; ++r) most = std::max(most, a.p[r].M);
   return most <= 64 ? la_simt_run<T, S, 64>(a, roles, st) : la_simt_run<T, S, 128>(a, roles, st);
 }
 
-// One chunk of the CUDA-core kernels: as fast there as on the tensor cores (B=1, H=4, D=64, T=1: 9.2 against 11.4 us;
-// T=64: 16.1 against 10.3), and where an output is a sum of a few terms, the rounding of their weights to bfloat16
-// would not average out.
-constexpr int64_t kLaShort = LaGeom<float>::C;
-
-template <class T, class S>
-static LaPath la_path(LaTcArgs* k, const LaArgs<S>& a, int roles) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    if (a.T > kLaShort) return la_tc_setup(k, a, roles) ? kLaTc : kLaMma;
-  return kLaSimt;
-}
-
 static void la_strides(int64_t (&d)[3], const int64_t* s) { for (int i = 0; i < 3; ++i) d[i] = s[i]; }
 
 template <class T, class S>
-static int la_fwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs,
-                  const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
-                  const int64_t* gs, LaLengths lengths, const void* init, double scale, void* o, int o_wide, void* fin,
-                  void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
+static int la_fwd(const LaSize& z, LaOperands x, const void* g, const int64_t* gs, LaLengths lengths, const void* init,
+                  double scale, int copies, void* o, int o_wide, void* fin, void* ws, int64_t wsb, uint32_t* status,
+                  cudaStream_t st) {
+  const bool tc = la_tensor_cores<T>(z.T);
+  const LaPlan l = la_plan_of<S>(tc, z, 1, false, copies);
+  if (l.total && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total)) return PTB_ERR_WORKSPACE;
+  if (tc)
+    if (int rc = la_copy_in(&x, copies, z, l, ws, st)) return rc;
   LaArgs<S> a = {};
   LaPass<S>& p = a.p[0];
-  p.x = q; p.y = k; p.z = v;
-  la_strides(p.xs, qs); la_strides(p.ys, ks); la_strides(p.zs, vs);
+  p.x = x.p[0]; p.y = x.p[1]; p.z = x.p[2];
+  la_strides(p.xs, x.st[0]); la_strides(p.ys, x.st[1]); la_strides(p.zs, x.st[2]);
   p.o = o;
   p.init = static_cast<const S*>(init);
   p.fin = static_cast<S*>(fin);
-  p.M = (int)Dk; p.N = (int)Dv;
+  p.M = (int)z.Dk; p.N = (int)z.Dv;
   p.po = (S)scale; p.pz = (S)1;
   p.wide = o_wide;
   a.g = static_cast<const S*>(g);
   la_strides(a.gs, gs);
   a.lengths = lengths;
-  a.B = B; a.T = T_; a.H = H;
-  LaTcArgs tc = {};
-  const LaPath path = la_path<T, S>(&tc, a, 1);
-  const LaPlan l = la_plan_of<S>(path, {B, T_, H, Dk, Dv}, 1, false);
-  if (l.total && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total)) return PTB_ERR_WORKSPACE;
-  return la_run<T, S>(a, &tc, path, 1, l, ws, status, st);
+  a.B = z.B; a.T = z.T; a.H = z.H;
+  return la_run<T, S>(a, 1, l, ws, status, st);
 }
 
 template <class T, class S>
-static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs,
-                  const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
-                  const int64_t* gs, LaLengths lengths, const void* init, double scale, const void* go,
-                  const int64_t* gos, const void* gfin, void* gq, void* gk, void* gv, void* gg, int gg_per_token,
+static int la_bwd(const LaSize& z, LaOperands op, const void* g, const int64_t* gs, LaLengths lengths, const void* init,
+                  double scale, int copies, const void* gfin, void* gq, void* gk, void* gv, void* gg, int gg_per_token,
                   void* ginit, void* ws, int64_t wsb, uint32_t* status, cudaStream_t st) {
-  const bool dec = gg != nullptr;
+  const bool dec = gg != nullptr, tc = la_tensor_cores<T>(z.T);
+  const int64_t B = z.B, H = z.H, Dk = z.Dk, Dv = z.Dv;
+  if (!gq && !gk && !gv && !dec && !ginit) return PTB_OK;
+  const LaPlan l = la_plan_of<S>(tc, z, 3, dec, copies);
+  if (l.total && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total)) return PTB_ERR_WORKSPACE;
+  if (tc)
+    if (int rc = la_copy_in(&op, copies, z, l, ws, st)) return rc;
+  const void *q = op.p[0], *k = op.p[1], *v = op.p[2], *go = op.p[3];
+  const int64_t *qs = op.st[0], *ks = op.st[1], *vs = op.st[2], *gos = op.st[3];
   char* w = static_cast<char*>(ws);
   LaArgs<S> a = {};
   a.g = static_cast<const S*>(g);
   la_strides(a.gs, gs);
   a.lengths = lengths;
-  a.B = B; a.T = T_; a.H = H;
+  a.B = B; a.T = z.T; a.H = H;
   int roles = 0;
   if (gq || dec) {
     LaPass<S>& p = a.p[roles++];
@@ -386,7 +400,7 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
     LaPass<S>& p = a.p[roles++];
     p.x = v; p.y = go; p.z = q; p.w = k;
     la_strides(p.xs, vs); la_strides(p.ys, gos); la_strides(p.zs, qs); la_strides(p.ws, ks);
-    p.o = gk;
+    p.o = gk; p.out = 1;
     p.init = static_cast<const S*>(gfin);
     p.fin = static_cast<S*>(ginit);
     p.M = (int)Dv; p.N = (int)Dk; p.state_t = 1; p.reverse = 1;
@@ -396,42 +410,36 @@ static int la_bwd(int64_t B, int64_t T_, int64_t H, int64_t Dk, int64_t Dv, cons
     LaPass<S>& p = a.p[roles++];
     p.x = k; p.y = q; p.z = go;
     la_strides(p.xs, ks); la_strides(p.ys, qs); la_strides(p.zs, gos);
-    p.o = gv;
+    p.o = gv; p.out = 2;
     p.init = static_cast<const S*>(gfin);
     p.M = (int)Dk; p.N = (int)Dv; p.reverse = 1;
     p.po = (S)1; p.pz = (S)scale;
   }
-  if (roles == 0) return PTB_OK;
-  LaTcArgs tc = {};
-  const LaPath path = la_path<T, S>(&tc, a, roles);
-  const LaPlan l = la_plan_of<S>(path, {B, T_, H, Dk, Dv}, 3, dec);
-  if (l.total && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) || wsb < l.total)) return PTB_ERR_WORKSPACE;
   if (dec) {   // the first two passes give what the gradient of the decays is made of
     a.p[0].bounds = reinterpret_cast<S*>(w + l.qb_off);
     a.p[0].dots = reinterpret_cast<S*>(w + l.qd_off);
     a.p[1].bounds = reinterpret_cast<S*>(w + l.rb_off);
     a.p[1].dots = reinterpret_cast<S*>(w + l.kd_off);
   }
-  if (int rc = la_run<T, S>(a, &tc, path, roles, l, ws, status, st)) return rc;
+  if (int rc = la_run<T, S>(a, roles, l, ws, status, st)) return rc;
   if (dec && l.nchunk > 0) {
     LaDecayArgs<S> d = {};
     d.s_bounds = reinterpret_cast<const S*>(w + l.qb_off);
     d.r_bounds = reinterpret_cast<const S*>(w + l.rb_off);
     d.qd = reinterpret_cast<const S*>(w + l.qd_off);
     d.kd = reinterpret_cast<const S*>(w + l.kd_off);
-    const int width = path == kLaMma ? kLaMaxDim : path == kLaTc ? kTcSlice : LaGeom<S>::NS, slices = (int)((Dk + width - 1) / width);
-    d.q_slices = d.k_slices = path == kLaTc ? 2 * slices : slices;   // there two warps share a row
+    const int width = tc ? kTcSlice : LaGeom<S>::NS, slices = (int)((Dk + width - 1) / width);
+    d.q_slices = d.k_slices = tc ? 2 * slices : slices;   // there two warps share a row
     d.g = a.g;
     la_strides(d.gs, gs);
     d.lengths = lengths;
-    d.B = B; d.T = T_; d.H = H; d.MN = l.bound_elems;
-    d.used = path == kLaTc ? (int64_t)slices * kTcSlice * kTcDim : l.bound_elems;   // columns a pass had
+    d.B = B; d.T = z.T; d.H = H; d.MN = l.bound_elems;
+    d.used = tc ? (int64_t)slices * kTcSlice * kTcDim : l.bound_elems;   // columns a pass had
     if (gg_per_token) d.dg = static_cast<S*>(gg);
     else d.part = reinterpret_cast<double*>(w + l.part_off);
     if (B * H * l.nchunk > 0x7fffffffll) return PTB_ERR_TOO_LARGE;
     const unsigned grid = (unsigned)(B * H * l.nchunk);
-    if (path == kLaTc) la_decay_grad_kernel<S, kTcChunk><<<grid, 256, 0, st>>>(d);
-    else if (path == kLaMma) la_decay_grad_kernel<S, kLaMmaChunk><<<grid, 256, 0, st>>>(d);
+    if (tc) la_decay_grad_kernel<S, kTcChunk><<<grid, 256, 0, st>>>(d);
     else la_decay_grad_kernel<S, LaGeom<S>::C><<<grid, 256, 0, st>>>(d);
     PTB_CUDA(cudaGetLastError());
   }
@@ -466,6 +474,7 @@ static int la_step(int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q, 
 static int la_check(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv) {
   if (dtype != PTB_F32 && dtype != PTB_F64 && dtype != PTB_F16 && dtype != PTB_BF16) return PTB_ERR_ARG;
   if (B < 0 || T < 0 || H < 0 || Dk < 1 || Dv < 1 || Dk > kLaMaxDim || Dv > kLaMaxDim) return PTB_ERR_ARG;
+  if (dtype == PTB_BF16 && T > 0x7fffff00ll) return PTB_ERR_TOO_LARGE;   // token numbers there, a chunk past the end too, in 32 bits
   if (B > 0x7fffffffll || H > 0x7fffffffll || B * H > 0x7fffffffll || T > (1ll << 40)) return PTB_ERR_TOO_LARGE;
   return PTB_OK;
 }
@@ -485,32 +494,32 @@ using namespace ptb;
 extern "C" {
 
 int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
-                                             int backward, int decay_grad) {
+                                             int backward, int decay_grad, int copies) {
   if (la_check(dtype, B, T, H, Dk, Dv) != PTB_OK) return 0;
   const LaSize z = {B, T, H, Dk, Dv};
   const int roles = backward ? 3 : 1;
-  if (dtype == PTB_F64) return la_plan_of<double>(kLaSimt, z, roles, decay_grad).total;
-  if (dtype != PTB_BF16 || T <= kLaShort) return la_plan_of<float>(kLaSimt, z, roles, decay_grad).total;
-  // which of the tensor-core kernels run depends on the operands' alignment too: room for either
-  return std::max(la_mma_plan(z, roles, decay_grad).total, la_tc_plan(z, roles, decay_grad).total);
+  PTB_LA_TYPES((la_plan_of<S_>(la_tensor_cores<T_>(T), z, roles, decay_grad, copies).total))
 }
 
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const void* lengths, int lengths_wide, const void* init, double scale, void* o, int o_wide, void* fin,
+                             const void* lengths, int lengths_wide, const void* init, double scale, int copies, void* o, int o_wide, void* fin,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
   if (int rc = la_check(dtype, B, T, H, Dk, Dv)) return rc;
   if (B == 0 || H == 0) return PTB_OK;
   if ((T > 0 && (!q || !k || !v || !o || !log_decay)) || !q_strides || !k_strides || !v_strides || !log_decay_strides) return PTB_ERR_ARG;
-  PTB_LA_TYPES((la_fwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
-                               LaLengths{lengths, lengths_wide}, init, scale, o, o_wide, fin, workspace, workspace_bytes, status, (cudaStream_t)stream)))
+  LaOperands x = {{q, k, v, nullptr}, {}};
+  la_strides(x.st[0], q_strides); la_strides(x.st[1], k_strides); la_strides(x.st[2], v_strides);
+  const LaSize z = {B, T, H, Dk, Dv};
+  PTB_LA_TYPES((la_fwd<T_, S_>(z, x, log_decay, log_decay_strides, LaLengths{lengths, lengths_wide}, init, scale, copies, o, o_wide,
+                               fin, workspace, workspace_bytes, status, (cudaStream_t)stream)))
 }
 
 int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,
                              const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
-                             const void* lengths, int lengths_wide, const void* init, double scale, const void* grad_o,
+                             const void* lengths, int lengths_wide, const void* init, double scale, int copies, const void* grad_o,
                              const int64_t* grad_o_strides, const void* grad_fin, void* grad_q, void* grad_k,
                              void* grad_v, void* grad_log_decay, int grad_log_decay_per_token, void* grad_init,
                              void* workspace, int64_t workspace_bytes, uint32_t* status, ptb_stream_t stream) {
@@ -519,10 +528,13 @@ int ptb_linear_attention_bwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t
   if ((T > 0 && (!q || !k || !v || !log_decay || !grad_o)) || !q_strides || !k_strides || !v_strides || !log_decay_strides ||
       !grad_o_strides)
     return PTB_ERR_ARG;
-  PTB_LA_TYPES((la_bwd<T_, S_>(B, T, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
-                               LaLengths{lengths, lengths_wide}, init, scale, grad_o, grad_o_strides, grad_fin, grad_q, grad_k, grad_v,
-                               grad_log_decay, grad_log_decay_per_token, grad_init, workspace, workspace_bytes,
-                               status, (cudaStream_t)stream)))
+  LaOperands x = {{q, k, v, grad_o}, {}};
+  la_strides(x.st[0], q_strides); la_strides(x.st[1], k_strides); la_strides(x.st[2], v_strides);
+  la_strides(x.st[3], grad_o_strides);
+  const LaSize z = {B, T, H, Dk, Dv};
+  PTB_LA_TYPES((la_bwd<T_, S_>(z, x, log_decay, log_decay_strides, LaLengths{lengths, lengths_wide}, init, scale, copies, grad_fin,
+                               grad_q, grad_k, grad_v, grad_log_decay, grad_log_decay_per_token, grad_init, workspace,
+                               workspace_bytes, status, (cudaStream_t)stream)))
 }
 
 int ptb_linear_attention_step(int dtype, int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q,

@@ -40,6 +40,7 @@ struct LaPass {
   S* dots;          // may be NULL: per token w[t].o[t] of the part inside the chunk and of the entering state,
                     //   [slice][bh][t][2]
   int M, N, state_t, reverse;
+  int out, pitch;   // tcgen05 kernels: which result o is, and its elements from row to row (a multiple of 8)
   int wide;         // o holds float32 beside a 2-byte type (for a normalisation that follows)
   S po, pz;
 };

@@ -11,9 +11,11 @@
 // and single warps drive the TMA loads (no multicast), the products and the running sums of the decays.  U of a
 // chunk does not wait for the state, so the chain from chunk to chunk is one multiply-add per element of the state.
 //
-// Accuracy as in linear_attention_mma.cuh: one rounding of P and of S to bfloat16 where the result is bfloat16; Zw in
-// two terms, three for a float32 final state; with DOTS (gradient of the decays) S and Zw in three terms, and the
-// pairs inside a chunk from the float32 scores themselves.
+// Accuracy.  q, k, v are exact operands; what the products take besides (weights inside a chunk, the weighted z, the
+// state) is float32 and has to be rounded.  For a bfloat16 RESULT one rounding of P and of S is as good as the
+// rounding of the result itself; Zw takes two bfloat16 terms (16 bits), because its rounding would meet that of S.  For
+// a float32 result (the final state, the gradient of the decays: DOTS) it is split into three terms (24 bits), and the
+// pairs inside a chunk come from the float32 scores themselves.
 //
 // Why this shape.  128 rows fill the tensor core; 64 columns leave room in shared memory (227 KB) for two stages of
 // X, Y and Z beside three terms of Zw, and in tensor memory for a second O and OI; the price is that both slices of
@@ -27,11 +29,26 @@
 // of the products alternate; tensor pipe 33 % busy, DRAM 29 %; with 128 SMs busy the 1000 W limit holds the clock at
 // 1.6 GHz.  183 us without the final state, 201 us with it (537 MB: floor 82 us).
 #pragma once
-#include "linear_attention_mma.cuh"
+#include "linear_attention.cuh"
 #include "packed.cuh"
 #include "tensor_map.cuh"
 
 namespace ptb {
+
+__device__ __forceinline__ uint32_t la_pack(float lo, float hi) {   // {lo, hi} in memory order
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// the two values of a packed pair, as float32
+__device__ __forceinline__ float la_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float la_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// exp of a difference of log decays given in units of log 2; results below the normal range are zero
+__device__ __forceinline__ float la_exp2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 constexpr int kTcChunk = 128, kTcSlice = 64, kTcDim = 128;
 constexpr int kTcPanel = kTcChunk * 128;            // bytes of 128 rows x 64 bfloat16
@@ -449,7 +466,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         if (part == 0) cs[row] = row_col;
       }
       const uint32_t pairs = rev ? ~0u << lane : ~0u >> (31 - lane);   // columns of the own block that count
-      const int64_t row_step = a.H * N, first_row = (b * a.T * a.H + h) * N + n0 + 32 * part;   // of the thread's columns
+      const int64_t row_step = a.H * p.pitch, first_row = (b * a.T * a.H + h) * p.pitch + n0 + 32 * part;   // of the thread's columns
       // a chunk's rows to memory
       auto out = [&](int i, float win, float pair_sum) {
         const int t = chunk_of(i) * C + row, n = valid(chunk_of(i)), sz = i & 1;
@@ -590,12 +607,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
       }
       // behind the sequence: zeros
       if (p.o) {
-        const int64_t first = (int64_t)(c0 + count) * C, stop = min(a.T, (int64_t)c1 * C);
+        const int64_t begin = (int64_t)(c0 + count) * C, stop = min(a.T, (int64_t)c1 * C);
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        const int pieces = min(8, (N - n0) / 8) * (WIDE ? 2 : 1), per = WIDE ? 4 : 8;
-        for (int64_t t = first + tid; t < stop; t += kTcRows)
+        const int pieces = min(8, (p.pitch - n0) / 8) * (WIDE ? 2 : 1), per = WIDE ? 4 : 8;
+        for (int64_t t = begin + tid; t < stop; t += kTcRows)
           for (int q = 0; q < pieces; ++q) {
-            const int64_t at = ((b * a.T + t) * a.H + h) * N + n0 + q * per;
+            const int64_t at = (b * a.T * a.H + h) * p.pitch + t * row_step + n0 + q * per;
             *reinterpret_cast<uint4*>(static_cast<char*>(p.o) + at * (16 / per)) = zero;
           }
       }
@@ -750,6 +767,60 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   if (warp == 16) tc_dealloc(tm, 512);
   if (tid == 0 && *gave_up && k.status) atomicOr(k.status, kErrPipelineWait);
   if (last_cta) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Entering states of the segments (slots [role][nseg + 1] of padded [n][m] matrices): seg[d+1] = exp(log decay of
+// segment d) * seg[d] + (what segment d added); with all_segments the last one is the final state.
+__global__ void la_tc_join_kernel(const LaArgs<float> a, int all_segments) {
+  const int role = blockIdx.y;
+  const LaPass<float>& p = a.p[role];
+  const int64_t BH = a.B * a.H, e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, bh = e / (kTcDim * kTcDim);
+  if (bh >= BH) return;
+  const int i = (int)(e % (kTcDim * kTcDim)), n = i / kTcDim, m = i % kTcDim;
+  const bool on = m < p.M && n < p.N;
+  const int64_t at = bh * p.M * p.N + (p.state_t ? n * p.M + m : m * p.N + n);
+  float v = p.init && on ? p.init[at] : 0.f;
+  const int count = a.nseg - (all_segments && p.fin ? 0 : 1);
+  for (int d = 0; d < count; ++d) {
+    const double lg = a.seg_log[(int64_t)(role * a.nseg + d) * BH + bh];
+    float* slot = a.seg + ((int64_t)(role * (a.nseg + 1) + d + 1) * BH + bh) * a.seg_stride + i;
+    v = expf((float)lg) * v + *slot;
+    *slot = v;
+  }
+  if (all_segments && p.fin && on) p.fin[at] = v;
+}
+
+// Rows moved between layouts: operands that the TMA unit cannot address (rows that do not start on 16 bytes) to rows
+// that do, and results from such rows to dense ones.  U: the widest access that all rows allow.  A CTA takes 64 rows,
+// whose starts it works out once; its threads then take neighbouring units, so that loads and stores are contiguous.
+// What lies between a row's end and the next one's start is never read.
+// Measured: q, k, v of B=4, T=2048, H=16, D=60 (8-byte units, 94 MB read and written) 22 us, o 7 us; B=4, T=512, H=8,
+// 65 and 127 channels (2-byte units) 11 us.
+constexpr int kLaMoveRows = 64;
+struct LaMoveArgs {
+  const char* src[4];
+  char* dst[4];
+  int64_t st[4][3], pitch[4];   // bytes: (B, T, H) strides of src, step from row to row of dst
+  int width[4];                 // bytes of a row
+  int64_t T, H, rows;
+};
+template <class U>
+__global__ void __launch_bounds__(256) la_move_kernel(const LaMoveArgs a) {
+  __shared__ int64_t start[kLaMoveRows];
+  const int k = blockIdx.y, tid = threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.x * kLaMoveRows;
+  const int rows = (int)min((int64_t)kLaMoveRows, a.rows - r0);
+  if (tid < rows) {
+    const int64_t r = r0 + tid, bt = r / a.H, h = r - bt * a.H, b = bt / a.T, t = bt - b * a.T;
+    start[tid] = b * a.st[k][0] + t * a.st[k][1] + h * a.st[k][2];
+  }
+  __syncthreads();
+  const unsigned units = a.width[k] / (int)sizeof(U);
+  char* const dst = a.dst[k] + r0 * a.pitch[k];
+  for (unsigned i = tid; i < rows * units; i += 256) {
+    const unsigned r = i / units, at = (i - r * units) * (unsigned)sizeof(U);
+    *reinterpret_cast<U*>(dst + r * a.pitch[k] + at) = *reinterpret_cast<const U*>(a.src[k] + start[r] + at);
+  }
 }
 
 }  // namespace ptb

@@ -55,8 +55,8 @@ def test_c_entry_points_refuse():
     p = ctypes.addressof(buf)
     s = I3(8, 8, 8)
 
-    def fwd(dtype=0, B=1, T=4, H=1, Dk=8, Dv=8, q=p, ws=None, wsb=0):
-        return lib.ptb_linear_attention_fwd(dtype, B, T, H, Dk, Dv, q, s, p, s, p, s, p, s, None, 0, None, 1.0, p, 0, None, ws, wsb,
+    def fwd(dtype=0, B=1, T=4, H=1, Dk=8, Dv=8, q=p, ws=None, wsb=0, copies=0):
+        return lib.ptb_linear_attention_fwd(dtype, B, T, H, Dk, Dv, q, s, p, s, p, s, p, s, None, 0, None, 1.0, copies, p, 0, None, ws, wsb,
                                             None, None)
 
     assert fwd(dtype=2) == 1 and fwd(dtype=9) == 1          # no complex numbers
@@ -65,13 +65,18 @@ def test_c_entry_points_refuse():
     # a row long enough to be cut needs a workspace, and it has to be aligned
     assert fwd(T=1 << 20) == 2 and fwd(T=1 << 20, ws=256, wsb=64) == 2 and fwd(T=1 << 20, ws=257, wsb=1 << 30) == 2
     assert fwd(B=0) == 0 and fwd(H=0) == 0
-    assert fwd(B=1 << 20, H=1 << 20) == 4
-    assert lib.ptb_linear_attention_workspace_bytes(0, 1, 4, 1, 8, 8, 0, 0) == 0
-    assert lib.ptb_linear_attention_workspace_bytes(0, 1, 1 << 20, 1, 8, 8, 0, 0) > 0
-    assert lib.ptb_linear_attention_workspace_bytes(2, 1, 4, 1, 8, 8, 0, 0) == 0
+    assert fwd(B=1 << 20, H=1 << 20) == 4 and fwd(dtype=5, T=0x7fffff01, ws=256, wsb=1 << 62) == 4
+    assert lib.ptb_linear_attention_workspace_bytes(0, 1, 4, 1, 8, 8, 0, 0, 0) == 0
+    assert lib.ptb_linear_attention_workspace_bytes(0, 1, 1 << 20, 1, 8, 8, 0, 0, 0) > 0
+    assert lib.ptb_linear_attention_workspace_bytes(2, 1, 4, 1, 8, 8, 0, 0, 0) == 0
+    # operands that have to be copied get their room
+    some = lib.ptb_linear_attention_workspace_bytes(5, 2, 100, 3, 33, 65, 0, 0, 0)
+    assert lib.ptb_linear_attention_workspace_bytes(5, 2, 100, 3, 33, 65, 0, 0, 7) >= some + 2 * 100 * 3 * (40 + 40 + 72) * 2
+    assert lib.ptb_linear_attention_workspace_bytes(0, 2, 100, 3, 33, 65, 0, 0, 7) == lib.ptb_linear_attention_workspace_bytes(
+        0, 2, 100, 3, 33, 65, 0, 0, 0)
     # the gradient of the decays keeps the states at the chunks' ends
-    plain = lib.ptb_linear_attention_workspace_bytes(5, 1, 4096, 4, 128, 128, 1, 0)
-    assert lib.ptb_linear_attention_workspace_bytes(5, 1, 4096, 4, 128, 128, 1, 1) >= plain + 2 * 32 * 4 * 128 * 128 * 4
+    plain = lib.ptb_linear_attention_workspace_bytes(5, 1, 4096, 4, 128, 128, 1, 0, 0)
+    assert lib.ptb_linear_attention_workspace_bytes(5, 1, 4096, 4, 128, 128, 1, 1, 0) >= plain + 2 * 32 * 4 * 128 * 128 * 4
     z = I2(8, 8)
     assert lib.ptb_linear_attention_step(0, 1, 1, 8, 200, p, z, p, z, p, z, p, z, 1.0, p, z, p, None) == 1
     assert lib.ptb_linear_attention_step(0, 1, 1, 8, 8, p, z, p, z, p, z, p, z, 1.0, None, z, p, None) == 1

@@ -32,6 +32,44 @@ def test_sizes(dtype, size, form):
     check_backward(form, list(some) + [None, None], *det, scale, None, go, gS)
 
 
+def place(t, how):
+    """The values of t (B,T,H,D) on rows that do not start on 16 bytes, or whose strides say so."""
+    B, T, H, D = t.shape
+    if how == "shifted":
+        return t.new_empty(t.numel() + 1)[1:].view(t.shape).copy_(t)
+    if how == "even":            # rows on 4 bytes
+        return t.new_empty(B, T, H, D + 2)[..., 2:].copy_(t)
+    if how == "heads first":     # memory order (H, B, T), an odd step from token to token
+        return t.new_empty(H, B, T, D + 3)[..., :D].permute(1, 2, 0, 3).copy_(t)
+    if how == "one token":
+        return t[:, :1].expand(B, T, H, D)
+    return t
+
+
+@pytest.mark.parametrize("forms", [("shifted", "", "", ""), ("", "even", "heads first", ""), ("one token", "", "shifted", "even"),
+                                   ("", "one token", "", "heads first"), ("even", "even", "even", "even"), ("", "", "", "one token")])
+@pytest.mark.parametrize("size", [(2, 140, 3, 64, 64), (1, 33, 1, 128, 72), (2, 400, 2, 36, 100), (1, 1200, 2, 7, 65)])
+def test_rows_off_the_boundaries(size, forms):
+    q, k, v, g, zi, scale = inputs(size, torch.bfloat16, "lpv", seed=26)
+    B, T, H, _ = q.shape
+    lengths = torch.tensor([T - 9] * B, device="cuda")
+    q, k, v = (place(t, how) for t, how in zip((q, k, v), forms))
+    leaves = [t.requires_grad_() for t in (q, k, v, g, zi)]
+    o, S = ptb.lpv.linear_attention(*leaves, scale=scale, lengths=lengths)
+    det = [t.detach() for t in leaves]
+    check_forward((o.detach(), S.detach()), *det, scale, lengths)
+    gen = torch.Generator(device="cuda").manual_seed(27)
+    go = place(torch.randn(o.shape, generator=gen, device="cuda").to(o.dtype), forms[3])
+    gS = torch.randn(S.shape, generator=gen, device="cuda").to(S.dtype)
+    check_backward("lpv", torch.autograd.grad([o, S], leaves, [go, gS], retain_graph=True), *det, scale, lengths, go, gS)
+    some = torch.autograd.grad([o, S], leaves[1:3], [go, gS])
+    check_backward("lpv", [None] + list(some) + [None, None], *det, scale, lengths, go, gS)
+    again = torch.autograd.grad(ptb.lpv.linear_attention(*leaves, scale=scale, lengths=lengths), leaves, [go, gS])
+    plain = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for t in leaves]
+    same = torch.autograd.grad(ptb.lpv.linear_attention(*plain, scale=scale, lengths=lengths), plain, [go.contiguous(), gS])
+    assert all(torch.equal(a, b) for a, b in zip(again, same))     # where the rows lie changes no bit
+
+
 @pytest.mark.parametrize("params", [True, False])
 @pytest.mark.parametrize("size", [(2, 20, 2, 32, 48), (2, 150, 3, 64, 128), (2, 90, 2, 33, 21), (1, 1500, 2, 128, 72)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
