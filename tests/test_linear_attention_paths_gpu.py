@@ -70,6 +70,47 @@ def test_rows_off_the_boundaries(size, forms):
     assert all(torch.equal(a, b) for a, b in zip(again, same))     # where the rows lie changes no bit
 
 
+def test_padded_batch_off_the_boundaries():
+    """Sequences of no token, of one, up to a chunk's end and behind it, NaN behind their ends; captured and replayed."""
+    q, k, v, g, zi, scale = inputs((5, 400, 2, 60, 33), torch.bfloat16, "lpv", seed=28)
+    lengths = torch.tensor([0, 1, 128, 129, 400], device="cuda")
+    clean = [t.clone() for t in (q, k, v, g)]
+    for t in (q, k, v, g):
+        for b, n in enumerate(lengths.tolist()):
+            t[b, n:] = float("nan")
+    leaves = [t.requires_grad_() for t in (q, k, v, g, zi)]
+    gen = torch.Generator(device="cuda").manual_seed(29)
+    go = torch.randn(v.shape, generator=gen, device="cuda").to(v.dtype)
+    gS = torch.randn(zi.shape, generator=gen, device="cuda")
+
+    def step():
+        o, S = ptb.lpv.linear_attention(*leaves, scale=scale, lengths=lengths)
+        return (o.detach(), S.detach()) + torch.autograd.grad([o, S], leaves, [go, gS])
+
+    first = step()
+    check_forward(first[:2], *clean, zi.detach(), scale, lengths)
+    check_backward("lpv", first[2:], *clean, zi.detach(), scale, lengths, go, gS)
+    with torch.no_grad():
+        y = ptb.lpv.linear_attention(*leaves[:4], scale=scale, lengths=lengths, norm_eps=1e-5)
+        for b, n in enumerate(lengths.tolist()):
+            assert (y[b, n:] == 0).all() and y[b, :n].isfinite().all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    del first
+    with torch.cuda.stream(side):
+        first = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(2):
+        for t in out:
+            t.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
+
+
 @pytest.mark.parametrize("params", [True, False])
 @pytest.mark.parametrize("size", [(2, 20, 2, 32, 48), (2, 150, 3, 64, 128), (2, 90, 2, 33, 21), (1, 1500, 2, 128, 72)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
