@@ -9,6 +9,7 @@ import ctypes
 import os
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # PHILTORCH_B200_LIB: load another build of the same library (kernel tuning experiments)
@@ -247,6 +248,13 @@ def eager(t: torch.Tensor) -> bool:
     dispatch mode, a functional transform) watching the dispatcher."""
     return (type(t) in _PLAIN and t.is_cuda and not torch.compiler.is_compiling() and not _dispatch_modes()
             and _transforms() is None)
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raises if one of the tensors carries a forward-mode tangent, for calls that have no rule for it: the kernels would run on
+    its primal alone, and the tangent would be lost without a word."""
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative (jvp): use reverse mode, or detach the tangent")
 
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)

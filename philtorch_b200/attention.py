@@ -325,6 +325,7 @@ def _norm_differentiable(*params: Optional[Tensor]) -> bool:
 def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tensor], scale: float,
            lengths: Optional[Tensor], return_state: Optional[bool], norm_eps: Optional[float],
            norm_weight: Optional[Tensor], norm_bias: Optional[Tensor]):
+    _lib.refuse_tangents("linear_attention", q, k, v, log_decay, zi, norm_weight, norm_bias)
     want = (zi is not None) if return_state is None else bool(return_state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or (zi is not None and zi.requires_grad)):
@@ -339,6 +340,7 @@ def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tens
 
 def attend_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, scale: float,
                 norm_eps: Optional[float], norm_weight: Optional[Tensor], norm_bias: Optional[Tensor]) -> Tensor:
+    _lib.refuse_tangents("linear_attention_step", q, k, v, log_decay, state, norm_weight, norm_bias)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or state.requires_grad):
         raise RuntimeError("linear_attention_step updates its state in place and is not differentiable: call it under "

@@ -36,7 +36,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Opt
 
     Returns:
         o (B, T, H, Dv), or (o, state).  Differentiable once in q, k, v, log_decay, zi (and the norm's
-        parameters).
+        parameters); forward-mode tangents are refused.
     """
     if log_decay.dim() != 3:
         raise ValueError(f"log_decay must be (batch, time, heads), got {tuple(log_decay.shape)}")

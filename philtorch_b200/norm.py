@@ -192,8 +192,9 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
     Returns:
         Tensor of x's shape and type.  Differentiable once in x, weight and bias; their gradients are sums
-        in a fixed order (bit-reproducible).
+        in a fixed order (bit-reproducible).  Forward-mode tangents are refused.
     """
+    _lib.refuse_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return LayerNorm.apply(x, weight, bias, float(eps), int(groups))
