@@ -39,18 +39,13 @@ constexpr int64_t kSmemPerSm = 228 * 1024, kSmemPerCtaMax = 227 * 1024, kSmemCta
 template <class S>
 static bool comb_tensor_map(CUtensorMap* map, const void* base, int64_t B, int64_t N, int64_t D, int64_t K, int W,
                             int KS) {
-  const EncodeTiledFn enc = tensor_map_encoder();
-  if (!enc || K < 1 || B < 1 || D > 0x7FFFFFFFll || K > 0x7FFFFFFFll || B > 0x7FFFFFFFll) return false;
+  if (K < 1 || B < 1 || D > 0x7FFFFFFFll || K > 0x7FFFFFFFll || B > 0x7FFFFFFFll) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)K, (cuuint64_t)B};
   const cuuint64_t strides[2] = {(cuuint64_t)D * sizeof(S), (cuuint64_t)N * sizeof(S)};   // bytes, multiples of 16
   if (strides[0] >= (1ull << 40) || strides[1] >= (1ull << 40)) return false;
   const cuuint32_t box[3] = {(cuuint32_t)W, (cuuint32_t)KS, 1u};
-  const cuuint32_t estr[3] = {1u, 1u, 1u};
-  const CUresult r = enc(map, sizeof(S) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 3,
-                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode_tiled(map, sizeof(S) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 3, base, dims,
+                      strides, box, CU_TENSOR_MAP_SWIZZLE_NONE) == CUDA_SUCCESS;
 }
 
 constexpr int kCombNoTensorMap = -1;   // the tensor maps could not be encoded: the caller uses the other kernels

@@ -140,8 +140,6 @@ static int la_simt_run(LaArgs<S>& a, int roles, cudaStream_t st) {
 // ---- tcgen05 kernels
 // (Dv | Dk, T, H, B) view of an operand, box 64 x 128 tokens; an axis of stride zero (or of one entry) is left out
 static int la_tc_map(LaTcMap* m, const void* base, const int64_t* st, int64_t B, int64_t T, int64_t H, int64_t D) {
-  const EncodeTiledFn enc = tensor_map_encoder();
-  if (!enc) return PTB_ERR_CUDA;
   m->bmul = B > 1 && st[0] != 0;
   m->hmul = H > 1 && st[2] != 0;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)(m->hmul ? H : 1), (cuuint64_t)(m->bmul ? B : 1)};
@@ -149,10 +147,11 @@ static int la_tc_map(LaTcMap* m, const void* base, const int64_t* st, int64_t B,
   if (!aligned16(base) || st[1] == 0) return PTB_ERR_ARG;
   for (cuuint64_t v : strides)
     if (v % 16 || v >= (1ull << 40)) return PTB_ERR_ARG;
-  const cuuint32_t box[4] = {64u, (cuuint32_t)kTcChunk, 1u, 1u}, estr[4] = {1u, 1u, 1u, 1u};
-  return enc(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? PTB_OK : PTB_ERR_ARG;
+  const cuuint32_t box[4] = {64u, (cuuint32_t)kTcChunk, 1u, 1u};
+  const CUresult r = encode_tiled(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (r == CUDA_SUCCESS) return PTB_OK;
+  g_last_cuda_error = (int)r;
+  return PTB_ERR_CUDA;
 }
 
 static int la_tc_setup(LaTcArgs* k, const LaArgs<float>& a, int roles) {

@@ -9,7 +9,7 @@ namespace ptb {
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// NULL where the driver has none: the caller uses kernels without tensor maps
+// NULL where the driver has none
 static EncodeTiledFn tensor_map_encoder() {
   static EncodeTiledFn fn = nullptr;
   static bool tried = false;
@@ -23,6 +23,23 @@ static EncodeTiledFn tensor_map_encoder() {
       fn = reinterpret_cast<EncodeTiledFn>(sym);
   }
   return fn;
+}
+
+// The encoder wants a context on the calling thread, which a thread has only from its first runtime call that needs one: an
+// autograd thread whose tensors all come from the allocator's cache has made none yet.  cudaSetDevice binds it.
+static CUresult encode_tiled(CUtensorMap* map, CUtensorMapDataType type, cuuint32_t rank, const void* base, const cuuint64_t* dims,
+                             const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  const EncodeTiledFn enc = tensor_map_encoder();
+  if (!enc) return CUDA_ERROR_NOT_FOUND;
+  const cuuint32_t estr[5] = {1u, 1u, 1u, 1u, 1u};
+  CUresult r = CUDA_SUCCESS;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    r = enc(map, type, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    int dev = 0;
+    if (r == CUDA_SUCCESS || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) break;
+  }
+  return r;
 }
 
 }  // namespace ptb
