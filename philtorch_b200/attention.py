@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import lib, ptr
-from .norm import layer_norm, layer_norm_of_sums
+from .norm import check_parameters, layer_norm, layer_norm_of_sums
 from .ops import _LIB, _TAGS
 
 __all__ = ["LinearAttention", "MAX_HEAD_DIM"]
@@ -308,9 +308,18 @@ class LinearAttention(Function):
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_o, grad_state)
 
 
-def _normalised(o: Tensor, dtype: torch.dtype, eps: Optional[float], weight: Optional[Tensor], bias: Optional[Tensor]) -> Tensor:
+def _check_norm(v: Tensor, eps: Optional[float], weight: Optional[Tensor], bias: Optional[Tensor]) -> None:
+    """What the norm of the read-out would refuse, before anything runs: a step has moved its state on by then."""
     if eps is None:
-        raise ValueError("norm_weight and norm_bias need norm_eps")
+        if weight is not None or bias is not None:
+            raise ValueError("norm_weight and norm_bias need norm_eps")
+    elif v.dim() >= 2:      # (anything else is refused by the operator's own checks)
+        check_parameters(v.shape[-2] * v.shape[-1], v.dtype, weight, bias, v.shape[-2])
+        if v.is_cuda:
+            _lib.require_cuda(v, weight, bias)
+
+
+def _normalised(o: Tensor, dtype: torch.dtype, eps: float, weight: Optional[Tensor], bias: Optional[Tensor]) -> Tensor:
     H, Dv = o.shape[-2:]
     rows = o.flatten(-2)
     if o.dtype == dtype:
@@ -326,6 +335,7 @@ def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tens
            lengths: Optional[Tensor], return_state: Optional[bool], norm_eps: Optional[float],
            norm_weight: Optional[Tensor], norm_bias: Optional[Tensor]):
     _lib.refuse_tangents("linear_attention", q, k, v, log_decay, zi, norm_weight, norm_bias)
+    _check_norm(v, norm_eps, norm_weight, norm_bias)
     want = (zi is not None) if return_state is None else bool(return_state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or (zi is not None and zi.requires_grad)):
@@ -333,7 +343,7 @@ def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tens
     else:   # (without gradients the normalisation reads the sums before they are rounded to q's type)
         wide = norm_eps is not None and not _norm_differentiable(norm_weight, norm_bias)
         o, state = _forward(q, k, v, log_decay, zi, lengths, float(scale), want, wide)
-    if norm_eps is not None or norm_weight is not None or norm_bias is not None:
+    if norm_eps is not None:
         o = _normalised(o, q.dtype, norm_eps, norm_weight, norm_bias)
     return (o, state) if want else o
 
@@ -341,6 +351,7 @@ def attend(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Optional[Tens
 def attend_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, scale: float,
                 norm_eps: Optional[float], norm_weight: Optional[Tensor], norm_bias: Optional[Tensor]) -> Tensor:
     _lib.refuse_tangents("linear_attention_step", q, k, v, log_decay, state, norm_weight, norm_bias)
+    _check_norm(v, norm_eps, norm_weight, norm_bias)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or state.requires_grad):
         raise RuntimeError("linear_attention_step updates its state in place and is not differentiable: call it under "
@@ -349,6 +360,6 @@ def attend_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tenso
         _lib.require_cuda(q)
     run = _linear_attention_step if _lib.eager(q) else _ops.linear_attention_step
     o = run(q, k, v, log_decay, state, float(scale))
-    if norm_eps is not None or norm_weight is not None or norm_bias is not None:
+    if norm_eps is not None:
         o = _normalised(o, q.dtype, norm_eps, norm_weight, norm_bias)
     return o

@@ -26,30 +26,33 @@ _LIB.define("layer_norm_bwd(Tensor x, Tensor? weight, Tensor? bias, Tensor stats
             "bool need_x, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)", tags=_TAGS)
 
 
-def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, out: Optional[torch.dtype] = None) -> None:
+def check_parameters(C: int, dtype: torch.dtype, weight: Optional[Tensor], bias: Optional[Tensor], groups: int,
+                     out: Optional[torch.dtype] = None) -> None:
+    """Whether rows of C channels of ``dtype`` can be normalised with these parameters (results in ``out``)."""
     # the common case in one expression: the explanations below cost more host time than the launch
-    if x.dim() >= 1 and 1 <= groups <= 65535:
-        C, dt = x.shape[-1], x.dtype if out is None else out
-        if (C and C % groups == 0 and C // groups <= MAX_WIDTH
-                and (weight is None or (weight.shape == (C,) and weight.dtype == dt))
-                and (bias is None or (bias.shape == (C,) and bias.dtype == dt)) and (out is None or x.dtype in (dt, torch.float32))):
-            return
-    torch._check(x.dim() >= 1, lambda: "x must have at least one axis")
-    C = x.shape[-1]
+    dt = dtype if out is None else out
+    if (1 <= groups <= 65535 and C and C % groups == 0 and C // groups <= MAX_WIDTH
+            and (weight is None or (weight.shape == (C,) and weight.dtype == dt))
+            and (bias is None or (bias.shape == (C,) and bias.dtype == dt)) and (out is None or dtype in (dt, torch.float32))):
+        return
     torch._check(1 <= groups <= 65535 and C % groups == 0 and C > 0,
                  lambda: f"the last axis ({C}) must be a multiple of groups ({groups}, at most 65535)")
     torch._check(C // groups <= MAX_WIDTH, lambda: f"groups of {C // groups} channels: the kernels cover 1..{MAX_WIDTH}.")
-    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
-    out = x.dtype if out is None else out
-    torch._check(out == x.dtype or (x.dtype == torch.float32 and out in (torch.float16, torch.bfloat16)),
-                 lambda: f"no results in {out} of {x.dtype} tensors")
+    wide = torch.float64 if dtype == torch.float64 else torch.float32
+    torch._check(dt == dtype or (dtype == torch.float32 and dt in (torch.float16, torch.bfloat16)),
+                 lambda: f"no results in {dt} of {dtype} tensors")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None:
             torch._check(tuple(p.shape) == (C,), lambda: f"{name} must be ({C},), got {tuple(p.shape)}")
-            torch._check(p.dtype in (out, wide), lambda: f"{name} must be {out} or {wide}, got {p.dtype}")
+            torch._check(p.dtype in (dt, wide), lambda: f"{name} must be {dt} or {wide}, got {p.dtype}")
     if weight is not None and bias is not None:
         torch._check(weight.dtype == bias.dtype,
                      lambda: f"weight and bias must have the same type, got {weight.dtype} and {bias.dtype}")
+
+
+def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, out: Optional[torch.dtype] = None) -> None:
+    torch._check(x.dim() >= 1, lambda: "x must have at least one axis")
+    check_parameters(x.shape[-1], x.dtype, weight, bias, groups, out)
 
 
 def _code(t: Tensor) -> int:
