@@ -188,7 +188,7 @@ __host__ __device__ constexpr uint32_t tc_idesc(int m, int n, bool a_mn, bool b_
 // for decays below one.
 struct __align__(16) TcFactors {
   float before[4], over[4], after[4];
-  float dec[2];   // over the chunk, in two floats: a rounded factor would count once a chunk
+  float dec[2];   // over the chunk, in two floats
 };
 __device__ __forceinline__ void tc_logs(float* Gs, TcFactors* f, const float (&raw)[4], bool rev, int lane, double* total) {
   constexpr double kLog2E = 1.4426950408889634;
@@ -222,10 +222,9 @@ __device__ __forceinline__ void tc_logs(float* Gs, TcFactors* f, const float (&r
       run += end[k];
       f->after[k] = la_exp2((float)(E - run));
     }
-    // 1 + (e^x - 1) keeps its error relative to the decay's distance from one
-    const float x = (float)(E * 0.69314718055994531), q = expm1f(x), one = 1.f + q;
-    f->dec[0] = x < -1.f ? expf(x) : one;
-    f->dec[1] = x < -1.f ? 0.f : q - (one - 1.f);
+    const LaDecay<float> dec(E * 0.69314718055994531);
+    f->dec[0] = dec.hi;
+    f->dec[1] = dec.lo;
   }
   *total += E;
 }
@@ -781,11 +780,20 @@ __global__ void la_tc_join_kernel(const LaArgs<float> a, int all_segments) {
   const int64_t at = bh * p.M * p.N + (p.state_t ? n * p.M + m : m * p.N + n);
   float v = p.init && on ? p.init[at] : 0.f;
   const int count = a.nseg - (all_segments && p.fin ? 0 : 1);
+  const double* log = a.seg_log + (int64_t)role * a.nseg * BH + bh;
+  float* slot = a.seg + ((int64_t)(role * (a.nseg + 1) + 1) * BH + bh) * a.seg_stride + i;
+  double lg = *log;
+  float more = *slot;
   for (int d = 0; d < count; ++d) {
-    const double lg = a.seg_log[(int64_t)(role * a.nseg + d) * BH + bh];
-    float* slot = a.seg + ((int64_t)(role * (a.nseg + 1) + d + 1) * BH + bh) * a.seg_stride + i;
-    v = expf((float)lg) * v + *slot;
-    *slot = v;
+    const LaDecay<float> dec = LaDecay<float>::of_chunk(lg);
+    const float add = more;
+    float* const at = slot;
+    if (d + 1 < count) {   // the next segment's values are on their way while this one's are worked on
+      lg = *(log += BH);
+      more = *(slot += BH * a.seg_stride);
+    }
+    v = dec(v, add);
+    *at = v;
   }
   if (all_segments && p.fin && on) p.fin[at] = v;
 }
