@@ -10,8 +10,8 @@
 //   dk: x=v,  y=do, z=q  mirrored    dv: x=k,  y=q,  z=do  mirrored
 // so the backward pass is one launch with the three of them side by side (they share their reads in L2).
 //
-// Weights are exponentials of DIFFERENCES of sums held in double, never ratios of exponentials: a decay of
-// zero (g = -inf, taken as -1e5) or a long row does not overflow or cancel.
+// Weights are exponentials of DIFFERENCES of sums held in double (in two doubles for float64), never ratios of exponentials: a
+// decay of zero (g = -inf, taken as -1e5) or a long row does not overflow or cancel.
 #pragma once
 #include "launch.cuh"
 
@@ -129,20 +129,39 @@ template <> struct LaDecay<double> {
   __device__ __forceinline__ bool single() const { return true; }
 };
 
-// Inclusive running sums of a chunk's log decays: G[i] for i < C, tokens from n on count 0.  One warp.
+// Inclusive running sums of a chunk's log decays: G[i] for i < C, tokens from n on count 0.  One warp.  With L, in two doubles G + L:
+// differences of sums behind a decay of zero (which is -1e5 in them) lose nothing.  float64 arithmetic needs that; beside
+// float32 one double is exact enough.
 template <class S, int C>
-__device__ __forceinline__ void la_running_logs(double* G, const S* g, int64_t t_stride, int64_t t0, int n, int lane) {
-  double carry = 0.0;
+__device__ __forceinline__ void la_running_logs(double* G, double* L, const S* g, int64_t t_stride, int64_t t0, int n, int lane) {
+  constexpr bool kTwo = std::is_same<S, double>::value;
+  double carry = 0.0, carry_lo = 0.0;
+  auto add = [](double& hi, double& lo, double h, double l) {   // lo takes what the rounding of hi + h loses
+    const double s = hi + h, t = s - hi;
+    lo += l + ((hi - (s - t)) + (h - t));
+    hi = s;
+  };
 #pragma unroll
   for (int i0 = 0; i0 < C; i0 += 32) {
     const int i = i0 + lane;
-    double v = i < n ? la_log(g[(t0 + i) * t_stride]) : 0.0;
+    double v = i < n ? la_log(g[(t0 + i) * t_stride]) : 0.0, lo = 0.0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const double u = __shfl_up_sync(0xffffffffu, v, d);
-      if (lane >= d) v += u;
+      if constexpr (kTwo) {
+        const double ul = __shfl_up_sync(0xffffffffu, lo, d);
+        if (lane >= d) add(v, lo, u, ul);
+      } else {
+        if (lane >= d) v += u;
+      }
     }
-    v += carry;
+    if constexpr (kTwo) {
+      add(v, lo, carry, carry_lo);
+      if (L) L[i] = lo;
+      carry_lo = __shfl_sync(0xffffffffu, lo, 31);
+    } else {
+      v += carry;
+    }
     G[i] = v;
     carry = __shfl_sync(0xffffffffu, v, 31);
   }
@@ -167,6 +186,7 @@ struct LaSimtSmem {
   // two chunks' decays: weight of the entering state per row, weight with which a token joins the state, running sums
   S win[2][C], wout[2][C];
   double G[2][C];
+  double L[2][sizeof(S) == 8 ? C : 1];
 };
 
 // Float32 / float64 arithmetic on the CUDA cores, any size up to 128: the path of float32, float64 and
@@ -182,6 +202,7 @@ __global__ void __launch_bounds__(256, sizeof(S) == 4 ? 2 : 1) la_simt_kernel(co
   constexpr int MR = MD * TN / 256;       // rows of the state per thread
   static_assert(MR >= 2 && C % 32 == 0, "thread tiles must cover the state");
   constexpr int TR = C / (256 / TN);      // rows of o per thread
+  constexpr bool kTwo = std::is_same<S, double>::value;   // sums of log decays in two doubles
   const int role = blockIdx.y;
   const LaPass<S>& p = a.p[role];
   const int slices = (p.N + NS - 1) / NS, seg_count = STATES_ONLY ? a.nseg - 1 : a.nseg;
@@ -225,11 +246,13 @@ __global__ void __launch_bounds__(256, sizeof(S) == 4 ? 2 : 1) la_simt_kernel(co
   // a chunk's decays, by one warp, a chunk ahead of their use
   auto decays = [&](int64_t ci, int buf) {
     const int64_t c = chunk_of(ci);
-    la_running_logs<S, C>(sm.G[buf], g, a.gs[1], c * C, valid(c), lane);
+    la_running_logs<S, C>(sm.G[buf], sm.L[buf], g, a.gs[1], c * C, valid(c), lane);
     __syncwarp();
     const double E = sm.G[buf][C - 1];
     for (int i = lane; i < C; i += 32) {
-      const S up = la_exp((S)sm.G[buf][i]), down = la_exp((S)(E - sm.G[buf][i]));
+      double to_end = E - sm.G[buf][i];
+      if constexpr (kTwo) to_end += sm.L[buf][C - 1] - sm.L[buf][i];
+      const S up = la_exp((S)sm.G[buf][i]), down = la_exp((S)to_end);
       sm.win[buf][i] = p.reverse ? down : up;
       sm.wout[buf][i] = (p.reverse ? up : down) * p.pz;
     }
@@ -337,7 +360,9 @@ __global__ void __launch_bounds__(256, sizeof(S) == 4 ? 2 : 1) la_simt_kernel(co
 #pragma unroll
           for (int j = 0; j < CS; ++j) {
             const int t = tr * CR + i, s = ts + TS * j;
-            const S w = la_exp((S)(p.reverse ? G[s] - G[t] : G[t] - G[s])) * p.pz;
+            double between = p.reverse ? G[s] - G[t] : G[t] - G[s];
+            if constexpr (kTwo) between += p.reverse ? sm.L[buf][s] - sm.L[buf][t] : sm.L[buf][t] - sm.L[buf][s];
+            const S w = la_exp((S)between) * p.pz;
             sm.p[t][s] = (p.reverse ? s >= t && s < n : s <= t) ? acc[i][j] * w : (S)0;
           }
       }
@@ -551,7 +576,7 @@ __global__ void __launch_bounds__(256) la_decay_grad_kernel(const LaDecayArgs<S>
   if (lane == 0) red[tid >> 5] = acc;
   __syncthreads();
   if (tid >= 32) return;
-  if (n > 0) la_running_logs<S, C>(G, a.g + b * a.gs[0] + h * a.gs[2], a.gs[1], t0, n, lane);
+  if (n > 0) la_running_logs<S, C>(G, nullptr, a.g + b * a.gs[0] + h * a.gs[2], a.gs[1], t0, n, lane);
   __syncwarp();
   double base = 0.0;
   for (int i = 0; i < 8; ++i) base += red[i];

@@ -1,11 +1,12 @@
-"""Linear attention: decays near one over long sequences (token by token, and chunk by chunk)."""
+"""Linear attention: decays near one over long sequences (token by token, and chunk by chunk), and decays of zero in
+float64, where a difference of large sums would show."""
 import math
 
 import pytest
 import torch
 
 import philtorch_b200 as ptb
-from test_linear_attention_gpu import inputs
+from test_linear_attention_gpu import check_backward, check_forward, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,19 @@ def test_an_infinite_state_stays_infinite(dtype):
     for got in (state[0], S[0, :2]):      # (a whole chunk's decay of exp(-80) times infinity is not asked for)
         assert (got[:, 2, 3] == float("inf")).all() and (got[:, 4, 5] == -float("inf")).all()
         assert got.isfinite().sum() == got.numel() - 2 * len(got)
+
+
+@pytest.mark.parametrize("zero", [-float("inf"), -1e4])
+def test_decay_of_zero_in_float64(zero):
+    """Weights behind a decay of zero are exponentials of differences of small sums: nothing of it is left in them."""
+    q, k, v, g, zi, scale = inputs((1, 300, 2, 64, 64), torch.float64, "lpv", seed=5)
+    for t in (0, 40, 41, 64, 128, 250):
+        g[:, t] = zero
+    leaves = [t.requires_grad_() for t in (q, k, v, g, zi)]
+    o, S = ptb.lpv.linear_attention(*leaves, scale=scale)
+    det = [t.detach() for t in leaves]
+    check_forward((o.detach(), S.detach()), *det, scale)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    go = torch.randn(o.shape, generator=gen, device="cuda", dtype=torch.float64)
+    gS = torch.randn(S.shape, generator=gen, device="cuda", dtype=torch.float64)
+    check_backward("lpv", torch.autograd.grad([o, S], leaves, [go, gS]), *det, scale, None, go, gS)
