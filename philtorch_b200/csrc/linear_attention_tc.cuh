@@ -76,7 +76,7 @@ struct LaTcSmem {
     zw = z + 2 * (dots ? 2 : 1) * kTcPanel;
     s = zw + nu * kTcPanel;
     misc = s + ns * kTcPanel;
-    total = misc + 2 * kTcChunk * 8 + kTcChunk * 4 + 2 * 64 + 192;
+    total = misc + 2 * kTcChunk * 8 + kTcChunk * 4 + 2 * 64 + 208;
   }
 };
 
@@ -202,7 +202,8 @@ __device__ __forceinline__ void tc_logs(float* Gs, TcFactors* f, const float (&r
     const double u = __shfl_up_sync(0xffffffffu, sum, d, 8);
     if ((lane & 7) >= d) sum += u;
   }
-  const double before = sum - v[3];
+  double before = __shfl_up_sync(0xffffffffu, sum, 1, 8);   // (not sum - v[3]: a NaN would reach the tokens before it)
+  if ((lane & 7) == 0) before = 0.0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const double in = rev ? -(before + v[j]) : before + v[j];
@@ -234,6 +235,42 @@ __device__ __forceinline__ void tc_load_logs(float (&raw)[4], const float* g, in
     const int i = 4 * lane + j;
     raw[j] = i < n ? g[(t0 + i) * t_stride] : 0.f;
   }
+}
+
+// An infinite or NaN value of z must not meet the zero weights of the tokens that do not see it (0 * inf): it is taken out of the
+// tile that P multiplies (Zw keeps it, so the state and everything behind the chunk get it), and the outputs that do see it become
+// NaN where they leave.  Both functions are out of line: they run on such data only.  What looking for it costs: prompt B=4, T=8192,
+// H=16, D=128 with a normalised read-out 281 -> 284 us; training step B=2, T=4096, H=16, D=128 345 -> 353 us.
+// Zeroes the odd values in the 32 columns of a row that a thread of the state group owns.
+__device__ __noinline__ void tc_take_out(unsigned char* z_row, int row, int part) {
+  for (int q = 4 * part; q < 4 * part + 4; ++q) {
+    uint4* const at = reinterpret_cast<uint4*>(z_row + ((q ^ (row & 7)) << 4));
+    uint4 v = *at;
+    uint32_t* const w = &v.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
+      if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu;
+    }
+    *at = v;
+  }
+}
+// Writes NaN to the columns n0 .. n0 + 31 of a row of o (the element o_at, if there is an o) that have an odd value in `rows` rows of z
+// from token t on; whether there is one.
+template <bool WIDE>
+__device__ __noinline__ bool tc_spoil(const LaPass<float>& p, int64_t b, int64_t h, int64_t t, int rows, int n0, int64_t o_at) {
+  const unsigned short* z = static_cast<const unsigned short*>(p.z) + b * p.zs[0] + h * p.zs[2] + t * p.zs[1] + n0;
+  const int columns = min(32, p.N - n0);
+  uint32_t odd = 0;
+  for (int r = 0; r < rows; ++r, z += p.zs[1])
+    for (int c = 0; c < columns; ++c)
+      if ((z[c] & 0x7f80u) == 0x7f80u) odd |= 1u << c;
+  for (int c = 0; c < columns; ++c)
+    if (p.o && odd >> c & 1) {
+      if (WIDE) static_cast<float*>(p.o)[o_at + c] = __int_as_float(0x7fffffff);
+      else static_cast<unsigned short*>(p.o)[o_at + c] = 0x7fffu;
+    }
+  return odd != 0;
 }
 
 // WIDE: o holds float32 (its own kernel: what a kernel's loops hold of code has to stay in the instruction cache)
@@ -284,6 +321,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   uint64_t *const lg_full = bars + 16, *const lg_empty = bars + 18;
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   volatile uint32_t* const gave_up = tmem_slot + 1;
+  // [4]: slot i & 3 holds i + 1 where z of chunk i has an infinite or NaN value (the state group is at most three chunks ahead of
+  // the rows that leave)
+  volatile int* const odd_chunk = reinterpret_cast<volatile int*>(tmem_slot + 2);
   // columns of tensor memory.  Without dots O and OI are double: a chunk's rows go out while the next one's weights are
   // formed; with dots the second scores take that place
   constexpr int kLag = DOTS ? 0 : 1;
@@ -314,6 +354,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     mbar_init(b_s, 8);
     mbar_init(b_oi, 1);
     *gave_up = 0;
+    for (int i = 0; i < 4; ++i) odd_chunk[i] = 0;
     fence_mbar_init();
   }
   tc_before();
@@ -471,7 +512,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         const int t = chunk_of(i) * C + row, n = valid(chunk_of(i)), sz = i & 1;
         const uint32_t at = lanes + (kLag ? (i & 1) * 64 : 0) + part * 32;
         const int64_t first = first_row + (int64_t)t * row_step;
-        const bool store = p.o && t < T;
+        const bool store = p.o && t < T, odd = odd_chunk[i & 3] == i + 1;
         TcPair ext(0.f, 0.f);
         const TcPair win2(win, win), scale2(scale_in, scale_in);
         uint32_t vi[2][16], vo[2][16];
@@ -514,6 +555,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
               }
             }
           }
+        }
+        if (odd) {   // of the tokens 0 .. row of the chunk, mirrored: row .. n - 1
+          if (row < n && tc_spoil<WIDE>(p, b, h, rev ? t : t - row, rev ? n - row : row + 1, n0 + 32 * part, first))
+            pair_sum = __int_as_float(0x7fffffff);
+          __syncwarp();
         }
         if (DOTS) {
           arrive_warp(zw_empty + sz);
@@ -687,7 +733,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
           }
         }
         unsigned char* const zw = tc_smem + L.zw + row * 128;
-        const TcPair wt2(wt, wt);
+        const TcPair wt2(wt, wt), zero2(0.f, 0.f);
+        TcPair odd(0.f, 0.f);   // stays zero unless a value is infinite or NaN
 #pragma unroll 1
         for (int q = 4 * part; q < 4 * part + 4; ++q) {
           const int at = (q ^ (row & 7)) << 4;
@@ -697,7 +744,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
           TcPair v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = tc_widen(in[e]) * wt2;
+            v[e] = tc_widen(in[e]);
+            if (!STATES_ONLY) odd = fma2(v[e], zero2, odd);
+            v[e] = v[e] * wt2;
             t[e] = tc_pack(v[e]);
           }
           *reinterpret_cast<uint4*>(zw + at) = make_uint4(t[0], t[1], t[2], t[3]);
@@ -711,6 +760,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = tc_pack(v[e] - tc_widen(t[e]));
             *reinterpret_cast<uint4*>(zw + 2 * kTcPanel + at) = make_uint4(t[0], t[1], t[2], t[3]);
+          }
+        }
+        if constexpr (!STATES_ONLY) {
+          const float2 f = odd.get();
+          if (!(f.x + f.y == 0.f)) {
+            tc_take_out(tc_smem + zoff, row, part);
+            odd_chunk[i & 3] = i + 1;
           }
         }
       }

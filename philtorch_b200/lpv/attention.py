@@ -31,8 +31,9 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Opt
             ``layer_norm`` (one group of Dv channels per head; weight and bias (H * Dv,)).
 
     bfloat16 tensors of more than 32 tokens run on the tensor cores: weights and states are rounded to bfloat16
-    once where they enter a product (sums, states and the decays' gradient are float32), and an infinite or NaN
-    value reaches the outputs of up to 127 tokens before it.
+    once where they enter a product (sums, states and the decays' gradient are float32), and an infinite value
+    counts as NaN.  Infinite and NaN values reach no output before their token and no gradient of q, k, v that does
+    not depend on them; in the gradient of log_decay they reach the chunk of tokens (up to 128) that they are in.
 
     Returns:
         o (B, T, H, Dv), or (o, state).  Differentiable once in q, k, v, log_decay, zi (and the norm's
