@@ -11,7 +11,7 @@ template <> struct LaGeom<double> { static constexpr int C = 32, NS = 32, PER_SM
 constexpr int kLaSms = 148;   // CTAs to aim for; only the cut of the time axis depends on it, never a result's meaning
 
 struct LaPlan {
-  int C, slices_max, nseg, seg_chunks;
+  int C, nseg, seg_chunks;
   int64_t nchunk, seg_off, log_off, qb_off, rb_off, qd_off, kd_off, part_off, total;
   int64_t seg_stride, bound_elems, copy_off[4], out_off[3];
 };
@@ -31,27 +31,28 @@ static void la_cut(int64_t ctas, int64_t nchunk, int64_t room, int64_t least, in
 
 struct LaSize { int64_t B, T, H, Dk, Dv; };
 
-// C: tokens of a chunk; width: columns of a state that a CTA takes; mn: scalars of a stored state
+// C: tokens of a chunk; width: columns of a state that a CTA takes; mn, bound: scalars of a segment's state and of one at a chunk's
+// end; groups: of threads that share a token's sum for the decays' gradient
 template <class S>
-static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int width, int64_t mn, int per_sm, int slots) {
+static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int width, int64_t mn, int64_t bound, int groups,
+                      int per_sm, int slots) {
   LaPlan l = {};
   l.C = C;
   const int64_t over_k = (z.Dk + width - 1) / width, over_v = (z.Dv + width - 1) / width;
-  l.slices_max = (int)std::max(over_k, over_v);
   const int64_t slices = roles == 1 ? over_v : 2 * over_k + over_v;   // of o; of dq, dk and dv
   l.nchunk = (z.T + C - 1) / C;
   const int64_t BH = z.B * z.H;
   la_cut(BH * slices, l.nchunk, kLaSms * per_sm, C == kTcChunk ? 3 : 2, &l.nseg, &l.seg_chunks);
   l.seg_stride = align_up(mn, 64);
-  l.bound_elems = mn;
+  l.bound_elems = bound;
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at = align_up(at + bytes, 256); return o; };
   l.seg_off = take(l.nseg > 1 ? (int64_t)roles * (l.nseg + slots) * BH * l.seg_stride * sizeof(S) : 0);
   l.log_off = take(l.nseg > 1 ? (int64_t)roles * l.nseg * BH * sizeof(double) : 0);
-  l.qb_off = take(decay_grad ? BH * l.nchunk * mn * sizeof(S) : 0);
-  l.rb_off = take(decay_grad ? BH * l.nchunk * mn * sizeof(S) : 0);
-  l.qd_off = take(decay_grad ? 2 * l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
-  l.kd_off = take(decay_grad ? 2 * l.slices_max * BH * z.T * 2 * sizeof(S) : 0);
+  l.qb_off = take(decay_grad ? BH * l.nchunk * bound * sizeof(S) : 0);
+  l.rb_off = take(decay_grad ? BH * l.nchunk * bound * sizeof(S) : 0);
+  l.qd_off = take(decay_grad ? groups * over_k * BH * z.T * 2 * sizeof(S) : 0);   // of the passes whose columns are Dk
+  l.kd_off = take(decay_grad ? groups * over_k * BH * z.T * 2 * sizeof(S) : 0);
   l.part_off = take(decay_grad ? BH * l.nchunk * sizeof(double) : 0);
   l.total = at;
   return l;
@@ -59,10 +60,10 @@ static LaPlan la_plan(const LaSize& z, int roles, bool decay_grad, int C, int wi
 template <class S>
 static LaPlan la_simt_plan(const LaSize& z, int roles, bool decay_grad) {
   using G = LaGeom<S>;
-  return la_plan<S>(z, roles, decay_grad, G::C, G::NS, z.Dk * z.Dv, G::PER_SM, 0);
+  return la_plan<S>(z, roles, decay_grad, G::C, G::NS, z.Dk * z.Dv, z.Dk * z.Dv, 1, G::PER_SM, 0);
 }
 static LaPlan la_tc_plan(const LaSize& z, int roles, bool decay_grad, int copies) {
-  LaPlan l = la_plan<float>(z, roles, decay_grad, kTcChunk, kTcSlice, kTcDim * kTcDim, 1, 1);
+  LaPlan l = la_plan<float>(z, roles, decay_grad, kTcChunk, kTcSlice, kTcDim * kTcDim, z.Dk * la_tc_bound_pitch((int)z.Dv), 2, 1, 1);
   auto take = [&](int64_t D, int size) {
     const int64_t o = l.total;
     l.total += align_up(z.B * z.T * z.H * align_up(D, 8) * size, 256);
@@ -433,7 +434,6 @@ static int la_bwd(const LaSize& z, LaOperands op, const void* g, const int64_t* 
     la_strides(d.gs, gs);
     d.lengths = lengths;
     d.B = B; d.T = z.T; d.H = H; d.MN = l.bound_elems;
-    d.used = tc ? (int64_t)slices * kTcSlice * kTcDim : l.bound_elems;   // columns a pass had
     if (gg_per_token) d.dg = static_cast<S*>(gg);
     else d.part = reinterpret_cast<double*>(w + l.part_off);
     if (B * H * l.nchunk > 0x7fffffffll) return PTB_ERR_TOO_LARGE;

