@@ -531,6 +531,11 @@ int ptb_linear_attention_step(int dtype, int64_t B, int64_t H, int64_t Dk, int64
                               const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                               const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
                               double scale, void* state, const int64_t* state_strides, void* o, ptb_stream_t stream);
+/* The same; o: (B,H,Dv) in the states' type, the sums before they are rounded (for a normalisation that follows). */
+int ptb_linear_attention_step_sums(int dtype, int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                                   const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                   const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                                   double scale, void* state, const int64_t* state_strides, void* o, ptb_stream_t stream);
 
 /* ---- layer norm over groups of channels --------------------------------------------------------
  * x: rows of groups * width channels (dense), x_stride elements apart; y dense, of y_dtype: x's, or PTB_F16 / PTB_BF16

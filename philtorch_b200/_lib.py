@@ -168,6 +168,8 @@ lib.ptb_linear_attention_bwd.restype = _i32
 lib.ptb_linear_attention_step.argtypes = ([_i32] + [_i64] * 4 + [_vp, _strides] * 4 + [ctypes.c_double, _vp, _strides, _vp]
                                           + [_vp])
 lib.ptb_linear_attention_step.restype = _i32
+lib.ptb_linear_attention_step_sums.argtypes = lib.ptb_linear_attention_step.argtypes
+lib.ptb_linear_attention_step_sums.restype = _i32
 lib.ptb_layer_norm_bwd_workspace_bytes.argtypes = [_i32] + [_i64] * 3
 lib.ptb_layer_norm_bwd_workspace_bytes.restype = _i64
 lib.ptb_layer_norm_fwd.argtypes = [_i32] + [_i64] * 3 + [_vp, _i64, _vp, _vp, _i32, ctypes.c_double, _i32] + [_vp] * 3 + [_vp]

@@ -136,8 +136,8 @@ _LIB.define("linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Te
 _LIB.define("linear_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? init, Tensor? lengths, "
             "float scale, Tensor? grad_o, Tensor? grad_state, bool need_q, bool need_k, bool need_v, "
             "bool need_decay, bool need_init) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", tags=_TAGS)
-_LIB.define("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, float scale) "
-            "-> Tensor", tags=_TAGS)
+_LIB.define("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, float scale, "
+            "bool wide=False) -> Tensor", tags=_TAGS)
 
 
 def _linear_attention(q, k, v, log_decay, init, lengths, scale, want_state, wide=False):
@@ -222,16 +222,16 @@ def _check_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, state: Tensor) -> No
                                                    f"apart from one another, got strides {tuple(state.stride())}")
 
 
-def _linear_attention_step(q, k, v, log_decay, state, scale):
+def _linear_attention_step(q, k, v, log_decay, state, scale, wide=False):
     _check_step(q, k, v, log_decay, state)
     dev = _lib.require_cuda(q, k, v, log_decay, state)
     B, H, Dk = q.shape
     Dv = v.shape[2]
     q, k, v = _rows(q), _rows(k), _rows(v)
-    o = v.new_empty((B, H, Dv))
+    o = (state if wide else v).new_empty((B, H, Dv))   # wide: in the sums' type, for a normalisation that follows
     if B and H:
         gs = _array((0, log_decay.stride(0)) if log_decay.dim() == 1 else log_decay.stride())
-        _lib.launch(lib.ptb_linear_attention_step, dev, _code(q), B, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k),
+        _lib.launch(lib.ptb_linear_attention_step_sums if wide else lib.ptb_linear_attention_step, dev, _code(q), B, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k),
                     _outer_strides(k), ptr(v), _outer_strides(v), ptr(log_decay), gs, scale, ptr(state),
                     _array(state.stride()[:2]), ptr(o))
         torch.autograd.graph.increment_version(state)
@@ -259,9 +259,9 @@ def _(q, k, v, log_decay, init, lengths, scale, grad_o, grad_state, need_q, need
 
 
 @torch.library.register_fake("philtorch_b200::linear_attention_step")
-def _(q, k, v, log_decay, state, scale):
+def _(q, k, v, log_decay, state, scale, wide=False):
     _check_step(q, k, v, log_decay, state)
-    return v.new_empty(v.shape)
+    return (state if wide else v).new_empty(v.shape)
 
 
 _ops = torch.ops.philtorch_b200
@@ -359,7 +359,8 @@ def attend_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tenso
     if q.device.type == "cpu":
         _lib.require_cuda(q)
     run = _linear_attention_step if _lib.eager(q) else _ops.linear_attention_step
-    o = run(q, k, v, log_decay, state, float(scale))
+    wide = norm_eps is not None and not _norm_differentiable(norm_weight, norm_bias)   # (as in attend)
+    o = run(q, k, v, log_decay, state, float(scale), wide)
     if norm_eps is not None:
         o = _normalised(o, q.dtype, norm_eps, norm_weight, norm_bias)
     return o

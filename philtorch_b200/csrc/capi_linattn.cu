@@ -453,13 +453,14 @@ static int la_bwd(const LaSize& z, LaOperands op, const void* g, const int64_t* 
 template <class T, class S>
 static int la_step(int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q, const int64_t* qs, const void* k,
                    const int64_t* ks, const void* v, const int64_t* vs, const void* g, const int64_t* gs, double scale,
-                   void* state, const int64_t* ss, void* o, cudaStream_t st) {
+                   void* state, const int64_t* ss, void* o, int o_wide, cudaStream_t st) {
   LaStepArgs<T, S> a;
   a.q = static_cast<const T*>(q); a.k = static_cast<const T*>(k); a.v = static_cast<const T*>(v);
   for (int i = 0; i < 2; ++i) { a.qs[i] = qs[i]; a.ks[i] = ks[i]; a.vs[i] = vs[i]; a.gs[i] = gs[i]; a.ss[i] = ss[i]; }
   a.g = static_cast<const S*>(g);
   a.state = static_cast<S*>(state);
-  a.o = static_cast<T*>(o);
+  a.o = o;
+  a.wide = o_wide;
   a.H = H; a.M = (int)Dk; a.N = (int)Dv;
   a.scale = (S)scale;
   constexpr int V = 16 / sizeof(S);
@@ -489,6 +490,18 @@ using namespace ptb;
     case PTB_F16: { using T_ = __half; using S_ = float; return CALL; }                      \
     default: { using T_ = __nv_bfloat16; using S_ = float; return CALL; }                    \
   }
+
+static int la_step_entry(int dtype, int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                         const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                         const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                         double scale, void* state, const int64_t* state_strides, void* o, int o_wide, ptb_stream_t stream) {
+  if (int rc = la_check(dtype, B, 1, H, Dk, Dv)) return rc;
+  if (B == 0 || H == 0) return PTB_OK;
+  if (!q || !k || !v || !log_decay || !state || !o || !q_strides || !k_strides || !v_strides || !log_decay_strides || !state_strides)
+    return PTB_ERR_ARG;
+  PTB_LA_TYPES((la_step<T_, S_>(B, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
+                                scale, state, state_strides, o, o_wide, (cudaStream_t)stream)))
+}
 
 extern "C" {
 
@@ -540,12 +553,16 @@ int ptb_linear_attention_step(int dtype, int64_t B, int64_t H, int64_t Dk, int64
                               const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                               const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
                               double scale, void* state, const int64_t* state_strides, void* o, ptb_stream_t stream) {
-  if (int rc = la_check(dtype, B, 1, H, Dk, Dv)) return rc;
-  if (B == 0 || H == 0) return PTB_OK;
-  if (!q || !k || !v || !log_decay || !state || !o || !q_strides || !k_strides || !v_strides || !log_decay_strides || !state_strides)
-    return PTB_ERR_ARG;
-  PTB_LA_TYPES((la_step<T_, S_>(B, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides,
-                                scale, state, state_strides, o, (cudaStream_t)stream)))
+  return la_step_entry(dtype, B, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides, scale, state,
+                       state_strides, o, 0, stream);
+}
+
+int ptb_linear_attention_step_sums(int dtype, int64_t B, int64_t H, int64_t Dk, int64_t Dv, const void* q,
+                                   const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                   const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                                   double scale, void* state, const int64_t* state_strides, void* o, ptb_stream_t stream) {
+  return la_step_entry(dtype, B, H, Dk, Dv, q, q_strides, k, k_strides, v, v_strides, log_decay, log_decay_strides, scale, state,
+                       state_strides, o, 1, stream);
 }
 
 }  // extern "C"

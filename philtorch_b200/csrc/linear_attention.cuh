@@ -656,9 +656,9 @@ struct LaStepArgs {
   int64_t gs[2];
   S* state;
   int64_t ss[2];
-  T* o;                          // dense (B,H,N)
+  void* o;                       // dense (B,H,N) of T, or of S when wide
   int64_t H;
-  int M, N;
+  int M, N, wide;
   S scale;
 };
 
@@ -707,7 +707,9 @@ __global__ void __launch_bounds__(256) la_step_kernel(const LaStepArgs<T, S> a) 
   if (tid < 32 && n0 + tid < a.N) {
     S sum = 0;
     for (int r = 0; r < RW; ++r) sum += red[r][tid];
-    la_store<T, S>(a.o + bh * a.N + n0 + tid, sum);
+    const int64_t at = bh * a.N + n0 + tid;
+    if (a.wide) static_cast<S*>(a.o)[at] = sum;
+    else la_store<T, S>(static_cast<T*>(a.o) + at, sum);
   }
 }
 

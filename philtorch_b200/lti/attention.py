@@ -28,7 +28,9 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, zi: Opt
             give zeros (a padded batch); values outside 0..T are clamped.
         return_state: whether the state after the last token is returned too; by default when zi is given.
         norm_eps, norm_weight, norm_bias: with norm_eps, the output of each head is normalised by
-            ``layer_norm`` (one group of Dv channels per head; weight and bias (H * Dv,)).
+            ``layer_norm`` (one group of Dv channels per head; weight and bias (H * Dv,)).  Without gradients it
+            reads the sums before they are rounded to q's type, with gradients the rounded output (the two operators
+            one after the other); the zeros behind a sequence's end become norm_bias.
 
     bfloat16 tensors of more than 32 tokens run on the tensor cores: weights and states are rounded to bfloat16
     once where they enter a product (sums, states and the decays' gradient are float32), and an infinite value
@@ -49,7 +51,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
                           norm_bias: Optional[Tensor] = None) -> Tensor:
     """One token of every sequence: ``state`` (B, H, Dk, Dv) moves on IN PLACE, and the token's output (B, H, Dv)
     is returned.  q, k: (B, H, Dk); v: (B, H, Dv); log_decay: (H,); the other arguments as in
-    ``linear_attention``.  Not differentiable (serving).
+    ``linear_attention`` (the norm reads the sums before they are rounded).  Not differentiable (serving).
     """
     if log_decay.dim() != 1:
         raise ValueError(f"log_decay must be (heads,), got {tuple(log_decay.shape)}")
