@@ -541,7 +541,7 @@ int ptb_linear_attention_step_sums(int dtype, int64_t B, int64_t H, int64_t Dk, 
  * x: rows of groups * width channels (dense), x_stride elements apart; y dense, of y_dtype: x's, or PTB_F16 / PTB_BF16
  * beside float32 x.  weight, bias: optional
  * (groups * width), of y's type, or float32 / float64 when params_wide.  mean, rstd: (rows, groups) in float32
- * (float64 beside PTB_F64), written by the forward call (both optional there) and read by the adjoint.
+ * (float64 beside PTB_F64), written by the forward call (there both or neither) and read by the adjoint.
  * 1 <= width <= 16384, groups <= 65535.  The parameter gradients have the parameters' type. */
 int64_t ptb_layer_norm_bwd_workspace_bytes(int dtype, int64_t rows, int64_t groups, int64_t width);
 int ptb_layer_norm_fwd(int dtype, int64_t rows, int64_t groups, int64_t width, const void* x, int64_t x_stride,

@@ -153,7 +153,7 @@ int ptb_layer_norm_fwd(int dtype, int64_t rows, int64_t groups, int64_t width, c
   if (int rc = ln_check(dtype, rows, groups, width)) return rc;
   if (y_dtype != dtype && !(dtype == PTB_F32 && (y_dtype == PTB_F16 || y_dtype == PTB_BF16))) return PTB_ERR_ARG;
   if (rows == 0) return PTB_OK;
-  if (!x || !y) return PTB_ERR_ARG;
+  if (!x || !y || !mean != !rstd) return PTB_ERR_ARG;
   PTB_LN_TYPES(LnArgs<S_> a = ln_args<S_>(rows, groups, width, x, x_stride, weight, bias, params_wide, mean, rstd);
                a.y = y; a.eps = (S_)eps; return (ln_fwd_to<T_, S_>(a, y_dtype, (cudaStream_t)stream));)
 }
