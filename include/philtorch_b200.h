@@ -503,11 +503,13 @@ int ptb_modal_bank_bwd(int dtype, int64_t rows, int64_t M, int64_t N, const void
  * int32, or int64 when lengths_wide, clamped to 0..T:
  * tokens from lengths[b] on are not read, leave the state alone and give zeros.  init, fin: optional dense
  * (B,H,Dk,Dv), the state before the first and after the last token.  o: dense (B,T,H,Dv), float32 when o_wide.
- * copies: PTB_BF16 and T > 32 only (else ignored): bit 0, 1, 2, 3 for q, k, v, grad_o.  Their rows have to start on
- * 16 bytes (base pointer 16-byte aligned; strides of axes longer than one a multiple of 8 elements, and not zero in
- * time); a marked operand need not, it is copied to the workspace first.  Unmarked and unaligned: PTB_ERR_ARG.
+ * copies: for sequences of more than ptb_linear_attention_any_rows_tokens(dtype) tokens (else ignored): bit 0, 1, 2, 3 for q, k,
+ * v, grad_o.  Their rows have to start on 16 bytes (base pointer 16-byte aligned; strides of axes longer than one a multiple of 8
+ * elements, and not zero in time); a marked operand need not, it is copied to the workspace first.  Unmarked and unaligned:
+ * PTB_ERR_ARG.  o and the gradients start on 16 bytes there.
  * workspace: ptb_linear_attention_workspace_bytes(..., backward, decay_grad, copies) bytes, 256-byte aligned, private to the
  * call until it completes; none (NULL) where that is 0.  status: as above (waits inside a CTA are bounded). */
+int64_t ptb_linear_attention_any_rows_tokens(int dtype);   /* INT64_MAX where any length takes rows anywhere */
 int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
                                              int backward, int decay_grad, int copies);
 int ptb_linear_attention_fwd(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, const void* q,

@@ -159,6 +159,8 @@ lib.ptb_lpv_biquad_tdf2_bwd.restype = _i32
 
 _strides = ctypes.POINTER(_i64)
 _la_in = [_i32] + [_i64] * 5 + [_vp, _strides] * 4 + [_vp, _i32, _vp, ctypes.c_double, _i32]
+lib.ptb_linear_attention_any_rows_tokens.argtypes = [_i32]
+lib.ptb_linear_attention_any_rows_tokens.restype = _i64
 lib.ptb_linear_attention_workspace_bytes.argtypes = [_i32] + [_i64] * 5 + [_i32] * 3
 lib.ptb_linear_attention_workspace_bytes.restype = _i64
 lib.ptb_linear_attention_fwd.argtypes = _la_in + [_vp, _i32, _vp] + _tail

@@ -114,9 +114,12 @@ def _workspace_bytes(*key) -> int:
     return n
 
 
+_ANY_ROWS = lib.ptb_linear_attention_any_rows_tokens(_lib.PTB_BF16)   # longer bfloat16 sequences run on the tensor cores
+
+
 def _copies(T: int, *tensors: Tensor) -> int:
     """The operands whose rows the tensor-core kernels' TMA loads cannot address, a bit for each: they are copied."""
-    if T <= 32 or tensors[0].dtype != torch.bfloat16:
+    if T <= _ANY_ROWS or tensors[0].dtype != torch.bfloat16:
         return 0
     mask = 0
     for i, t in enumerate(tensors):

@@ -90,9 +90,11 @@ static LaPlan la_plan_of(bool tensor_cores, const LaSize& z, int roles, bool dec
 // against 11.4 us; T=64: 16.1 against 10.3), and where an output is a sum of a few terms, the rounding of their
 // weights to bfloat16 would not average out.
 template <class T>
-static bool la_tensor_cores(int64_t tokens) {
-  return std::is_same<T, __nv_bfloat16>::value && tokens > LaGeom<float>::C;
+static int64_t la_cuda_core_tokens() {   // the most that they take
+  return std::is_same<T, __nv_bfloat16>::value ? LaGeom<float>::C : INT64_MAX;
 }
+template <class T>
+static bool la_tensor_cores(int64_t tokens) { return tokens > la_cuda_core_tokens<T>(); }
 
 template <class T, class S, int MD, bool STATES_ONLY>
 static int la_simt_launch(const LaArgs<S>& a, int roles, cudaStream_t st) {
@@ -504,6 +506,10 @@ static int la_step_entry(int dtype, int64_t B, int64_t H, int64_t Dk, int64_t Dv
 }
 
 extern "C" {
+
+int64_t ptb_linear_attention_any_rows_tokens(int dtype) {
+  return dtype == PTB_BF16 ? la_cuda_core_tokens<__nv_bfloat16>() : la_cuda_core_tokens<float>();
+}
 
 int64_t ptb_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv,
                                              int backward, int decay_grad, int copies) {

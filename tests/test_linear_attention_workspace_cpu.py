@@ -30,3 +30,18 @@ def test_small_heads_take_less_than_their_operands():
     operands = 4 * B * T * H * D * 2
     assert bytes_of(BF16, B, T, H, D, D, 1, 1, 0) < operands
     assert bytes_of(F32, B, T, H, D, D, 1, 1, 0) < 2 * operands
+
+
+def test_where_the_kernels_change_over_is_said_once():
+    """Operands on any rows are copied from one length on: the library's own, for the checks of the arguments and for the room."""
+    import torch
+    from philtorch_b200 import attention
+
+    last = _lib.lib.ptb_linear_attention_any_rows_tokens(BF16)
+    assert all(_lib.lib.ptb_linear_attention_any_rows_tokens(d) == 2 ** 63 - 1 for d in (F32, F64, F16))
+    for T in (last - 1, last, last + 1):
+        copied = bytes_of(BF16, 2, T, 3, 33, 65, 0, 0, 7) > bytes_of(BF16, 2, T, 3, 33, 65, 0, 0, 0)
+        assert copied == (T > last)
+        odd = torch.empty(2, T, 3, 33, dtype=torch.bfloat16)
+        assert attention._copies(T, odd, odd, odd) == (7 if T > last else 0)
+        assert attention._copies(T, *[t.float() for t in (odd, odd, odd)]) == 0
