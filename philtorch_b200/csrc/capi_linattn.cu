@@ -275,7 +275,7 @@ static int la_tc_launch(const LaTcArgs& k, int roles, cudaStream_t st, bool besi
   return PTB_OK;
 }
 
-// roles [0, exact) have dots
+// The roles with dots come first, then those without
 static int la_tc_run(LaTcArgs& k, int roles, cudaStream_t st) {
   const LaArgs<float>& a = k.a;
   bool dots = false;
@@ -288,7 +288,6 @@ static int la_tc_run(LaTcArgs& k, int roles, cudaStream_t st) {
   }
   if (a.nseg > 1) {
     k.xy_stages = 2;
-    k.dots = 0;
     if (int rc = la_tc_launch<true, false>(k, roles, st)) return rc;
     const int64_t elems = a.B * a.H * kTcDim * kTcDim;
     if (elems / 256 > 0x7fffffffll) return PTB_ERR_TOO_LARGE;

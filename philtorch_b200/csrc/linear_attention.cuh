@@ -190,7 +190,7 @@ struct LaSimtSmem {
 };
 
 // Float32 / float64 arithmetic on the CUDA cores, any size up to 128: the path of float32, float64 and
-// float16 tensors.  A CTA walks one (b, h, segment) in time order with a slice of NS columns of
+// float16 tensors, and of bfloat16 tensors of at most 32 tokens.  A CTA walks one (b, h, segment) in time order with a slice of NS columns of
 // the state in registers (8 x 4 per thread in float32) and a copy in shared memory for the products that read it.
 // Two CTAs an SM: one's barriers and loads lie under the other's arithmetic.
 template <class T, class S, int C, int NS, int MD, bool STATES_ONLY>

@@ -1,5 +1,5 @@
-// The passes of linear_attention.cuh on the fifth-generation tensor cores (tcgen05, accumulators in tensor memory), for
-// bfloat16 tensors with a head size above 64 whose rows the TMA unit can address.
+// The passes of linear_attention.cuh on the fifth-generation tensor cores (tcgen05, accumulators in tensor memory), for bfloat16
+// tensors of more than 32 tokens and any head size (operands that the TMA unit cannot address are copied first: la_move_kernel).
 //
 // A CTA walks one (b, h, segment) in chunks of 128 tokens with a slice of 64 columns of the state.  Four products per
 // chunk, issued by one thread:
@@ -66,7 +66,7 @@ struct LaTcArgs {
   LaArgs<float> a;
   LaTcMap x[3], y[3], z[3], w[3];
   int nu[3], ns[3];   // terms of Zw and of S
-  int xy_stages, dots, all_segments;
+  int xy_stages, all_segments;
   long long wait_cycles;
   uint32_t* status;
 };
