@@ -327,6 +327,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   // [4]: slot i & 3 holds i + 1 where z of chunk i has an infinite or NaN value (the state group is at most three chunks ahead of
   // the rows that leave)
   volatile int* const odd_chunk = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  uint64_t* const b_end = bars + 25;
   // columns of tensor memory.  Without dots O and OI are double: a chunk's rows go out while the next one's weights are
   // formed; with dots the second scores take that place
   constexpr int kLag = DOTS ? 0 : 1;
@@ -356,6 +357,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     mbar_init(b_u, 1);
     mbar_init(b_s, 8);
     mbar_init(b_oi, 1);
+    mbar_init(b_end, 1);
     *gave_up = 0;
     for (int i = 0; i < 4; ++i) odd_chunk[i] = 0;
     fence_mbar_init();
@@ -365,7 +367,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   tc_after();
   const uint32_t tm = *tmem_slot;
   // a wait that runs out lets every other wait of the CTA fall through: all warps reach the end, results are invalid
-  // and the status word says so
+  // and the status word says so.  No load is issued from then on: without the waits for their stages the loads would run away,
+  // past what a barrier counts
   auto wait = [&](uint64_t* bar, uint32_t parity) {   // by one thread; short code: it is in every loop
     if (mbar_try_wait(bar, parity)) return;
     const long long start = clock64();
@@ -384,10 +387,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
 
   if (warp == 17) {
     if (lane == 0) {   // loads
+      int xy_sent = 0, zw_sent = 0;
 #pragma unroll 1
       for (int i = 0; i < count; ++i) {
         const int t0 = chunk_of(i) * C, s = i % sxy, sz = i & 1;
         if (i >= sxy) wait(xy_empty + s, (i / sxy - 1) & 1);
+        if (*gave_up) break;
         const uint32_t X = base + s * 4 * kTcPanel, Y = X + 2 * kTcPanel;
         mbar_arrive_expect_tx(xy_full + s, (STATES_ONLY ? 2 : 4) * kTcPanel);
         for (int q = 0; q < 2; ++q) {
@@ -395,17 +400,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
             tc_tma(X + q * kTcPanel, &k.x[role].map, q * 64, t0, (int)h * k.x[role].hmul, (int)b * k.x[role].bmul, xy_full + s);
           tc_tma(Y + q * kTcPanel, &k.y[role].map, q * 64, t0, (int)h * k.y[role].hmul, (int)b * k.y[role].bmul, xy_full + s);
         }
+        xy_sent = i + 1;
         if (i >= 2) wait(zw_empty + sz, (i / 2 - 1) & 1);
+        if (*gave_up) break;
         const uint32_t Z = base + L.z + sz * (DOTS ? 2 : 1) * kTcPanel;
         mbar_arrive_expect_tx(zw_full + sz, (DOTS ? 2 : 1) * kTcPanel);
         tc_tma(Z, &k.z[role].map, n0, t0, (int)h * k.z[role].hmul, (int)b * k.z[role].bmul, zw_full + sz);
         if (DOTS) tc_tma(Z + kTcPanel, &k.w[role].map, n0, t0, (int)h * k.w[role].hmul, (int)b * k.w[role].bmul, zw_full + sz);
+        zw_sent = i + 1;
       }
       // nothing is on its way when the CTA ends, whatever its waits came to
-      for (int i = max(0, count - 2); i < count; ++i) {
-        if (i >= count - sxy && !mbar_wait_bounded(xy_full + i % sxy, (i / sxy) & 1, k.wait_cycles / 2)) *gave_up = 1;
+#pragma unroll 1
+      for (int i = max(0, xy_sent - sxy); i < xy_sent; ++i)
+        if (!mbar_wait_bounded(xy_full + i % sxy, (i / sxy) & 1, k.wait_cycles / 2)) *gave_up = 1;
+#pragma unroll 1
+      for (int i = max(0, zw_sent - 2); i < zw_sent; ++i)
         if (!mbar_wait_bounded(zw_full + (i & 1), (i / 2) & 1, k.wait_cycles / 2)) *gave_up = 1;
-      }
     }
   } else if (warp == 16) {
     {   // products: the warp stays together (operands in uniform registers), one thread issues
@@ -460,7 +470,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         if (one) tc_commit(zw_empty + sz);
         if (!STATES_ONLY && i + 1 < count) scores(i + 1);
       }
-      if (count > 0 && !mbar_wait_bounded(zw_empty + ((count - 1) & 1), ((count - 1) / 2) & 1, k.wait_cycles / 2)) *gave_up = 1;
+      if (one) tc_commit(b_end);   // every product has ended, whatever the waits came to
+      if (!mbar_wait_bounded(b_end, 0, k.wait_cycles / 2)) *gave_up = 1;
     }
   } else if (warp == 18) {   // decays
     float raw[4], next[4];
