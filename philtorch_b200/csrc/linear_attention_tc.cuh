@@ -25,9 +25,9 @@
 // Rows leaving a chunk later: 203 -> 178 us.  Tried and dropped: P in the place of the scores with U in one
 // product (194 us: the next scores then wait for O), loading the next scores ahead in registers (216 us),
 // prefetching tiles into L2 (no change), 32-byte stores (2.3 -> 3.1 us a chunk).
-// What bounds it: 2.3 us a chunk and CTA, in which the row group (weights 1.0, output 0.6 us) and the issue order
-// of the products alternate; tensor pipe 33 % busy, DRAM 29 %; with 128 SMs busy the 1000 W limit holds the clock at
-// 1.6 GHz.  183 us without the final state, 201 us with it (537 MB: floor 82 us).
+// What bounds it: 2.5 us a chunk and CTA, in which the row group (weights 1.0, output 0.6 us) and the issue order
+// of the products alternate; tensor pipe 29 % busy, DRAM 28 %; with 128 SMs busy the 1000 W limit may hold the clock at
+// 1.6 GHz.  157 us without the final state, 186 us with it (537 MB: floor 82 us); 183 and 201 us at 1.6 GHz.
 #pragma once
 #include "linear_attention.cuh"
 #include "packed.cuh"
