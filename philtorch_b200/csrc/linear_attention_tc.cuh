@@ -241,9 +241,10 @@ __device__ __forceinline__ void tc_load_logs(float (&raw)[4], const float* g, in
 }
 
 // An infinite or NaN value of z must not meet the zero weights of the tokens that do not see it (0 * inf): it is taken out of the
-// tile that P multiplies (Zw keeps it, so the state and everything behind the chunk get it), and the outputs that do see it become
-// NaN where they leave.  Both functions are out of line: they run on such data only.  What looking for it costs: prompt B=4, T=8192,
-// H=16, D=128 with a normalised read-out 281 -> 284 us; training step B=2, T=4096, H=16, D=128 345 -> 353 us.
+// tile that P multiplies (Zw keeps it, so the state and everything behind the chunk get it), and at the end the outputs that do see it
+// are overwritten with NaN.  Both functions are out of line: they run on such data only.  What looking for it costs: nothing for a
+// prompt of B=4, T=8192, H=16, D=128 (with a normalised read-out 281 us), 345 -> 349 us for a training step of B=2, T=4096, H=16, D=128.
+// (Rows that looked at each chunk as it left: 353 us; that replaced their values in registers: 366 us.)
 // Zeroes the odd values in the 32 columns of a row that a thread of the state group owns.
 __device__ __noinline__ void tc_take_out(unsigned char* z_row, int row, int part) {
   for (int q = 4 * part; q < 4 * part + 4; ++q) {
@@ -258,22 +259,38 @@ __device__ __noinline__ void tc_take_out(unsigned char* z_row, int row, int part
     *at = v;
   }
 }
-// Writes NaN to the columns n0 .. n0 + 31 of a row of o (the element o_at, if there is an o) that have an odd value in `rows` rows of z
-// from token t on; whether there is one.
-template <bool WIDE>
-__device__ __noinline__ bool tc_spoil(const LaPass<float>& p, int64_t b, int64_t h, int64_t t, int rows, int n0, int64_t o_at) {
-  const unsigned short* z = static_cast<const unsigned short*>(p.z) + b * p.zs[0] + h * p.zs[2] + t * p.zs[1] + n0;
-  const int columns = min(32, p.N - n0);
-  uint32_t odd = 0;
-  for (int r = 0; r < rows; ++r, z += p.zs[1])
-    for (int c = 0; c < columns; ++c)
-      if ((z[c] & 0x7f80u) == 0x7f80u) odd |= 1u << c;
-  for (int c = 0; c < columns; ++c)
-    if (p.o && odd >> c & 1) {
-      if (WIDE) static_cast<float*>(p.o)[o_at + c] = __int_as_float(0x7fffffff);
-      else static_cast<unsigned short*>(p.o)[o_at + c] = 0x7fffu;
+// Over the chunks c0 .. c0 + count - 1 again, by a warp of the row group: NaN to a thread's outputs (its row of each chunk, columns from n0
+// on, from the element o_at + t * o_step on) and dots that see an odd value of their chunk.
+template <bool DOTS, bool WIDE>
+__device__ __noinline__ void tc_spoil(const LaPass<float>& p, float* dots, int64_t b, int64_t h, int c0, int count, int len, int row,
+                                      int n0, int64_t o_at, int64_t o_step) {
+  const int columns = min(32, p.N - n0), lane = row & 31;
+  for (int c = c0; c < c0 + count; ++c) {
+    const int n = min(kTcChunk, len - c * kTcChunk);
+    const unsigned short* const z =
+        static_cast<const unsigned short*>(p.z) + b * p.zs[0] + h * p.zs[2] + (int64_t)c * kTcChunk * p.zs[1] + n0;
+    auto odd_in = [&](int r) {
+      uint32_t m = 0;
+      for (int j = 0; j < columns; ++j)
+        if ((z[r * p.zs[1] + j] & 0x7f80u) == 0x7f80u) m |= 1u << j;
+      return m;
+    };
+    uint32_t odd = 0;
+    for (int r = lane; r < n; r += 32) odd |= odd_in(r);
+    if (!__any_sync(0xffffffffu, odd != 0)) continue;
+    if (row < n) {   // it sees the tokens up to its own, mirrored: from its own on
+      odd = 0;
+      for (int r = p.reverse ? row : 0; r < (p.reverse ? n : row + 1); ++r) odd |= odd_in(r);
+      const int64_t t = (int64_t)c * kTcChunk + row;
+      for (int j = 0; j < columns; ++j)
+        if (p.o && odd >> j & 1) {
+          if (WIDE) static_cast<float*>(p.o)[o_at + t * o_step + j] = __int_as_float(0x7fffffff);
+          else static_cast<unsigned short*>(p.o)[o_at + t * o_step + j] = 0x7fffu;
+        }
+      if (DOTS && odd) dots[t * 2] = __int_as_float(0x7fffffff);
     }
-  return odd != 0;
+    __syncwarp();
+  }
 }
 
 // WIDE: o holds float32 (its own kernel: what a kernel's loops hold of code has to stay in the instruction cache)
@@ -324,10 +341,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
   uint64_t *const lg_full = bars + 16, *const lg_empty = bars + 18;
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   volatile uint32_t* const gave_up = tmem_slot + 1;
-  // [4]: slot i & 3 holds i + 1 where z of chunk i has an infinite or NaN value (the state group is at most three chunks ahead of
-  // the rows that leave)
-  volatile int* const odd_chunk = reinterpret_cast<volatile int*>(tmem_slot + 2);
-  uint64_t* const b_end = bars + 25;
+  volatile uint32_t* const odd_seen = tmem_slot + 2;   // some z had an infinite or NaN value
+  uint64_t* const b_end = bars + 24;
   // columns of tensor memory.  Without dots O and OI are double: a chunk's rows go out while the next one's weights are
   // formed; with dots the second scores take that place
   constexpr int kLag = DOTS ? 0 : 1;
@@ -359,7 +374,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
     mbar_init(b_oi, 1);
     mbar_init(b_end, 1);
     *gave_up = 0;
-    for (int i = 0; i < 4; ++i) odd_chunk[i] = 0;
+    *odd_seen = 0;
     fence_mbar_init();
   }
   tc_before();
@@ -526,7 +541,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         const int t = chunk_of(i) * C + row, n = valid(chunk_of(i)), sz = i & 1;
         const uint32_t at = lanes + (kLag ? (i & 1) * 64 : 0) + part * 32;
         const int64_t first = first_row + (int64_t)t * row_step;
-        const bool store = p.o && t < T, odd = odd_chunk[i & 3] == i + 1;
+        const bool store = p.o && t < T;
         TcPair ext(0.f, 0.f);
         const TcPair win2(win, win), scale2(scale_in, scale_in);
         uint32_t vi[2][16], vo[2][16];
@@ -569,11 +584,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
               }
             }
           }
-        }
-        if (odd) {   // of the tokens 0 .. row of the chunk, mirrored: row .. n - 1
-          if (row < n && tc_spoil<WIDE>(p, b, h, rev ? t : t - row, rev ? n - row : row + 1, n0 + 32 * part, first))
-            pair_sum = __int_as_float(0x7fffffff);
-          __syncwarp();
         }
         if (DOTS) {
           arrive_warp(zw_empty + sz);
@@ -664,6 +674,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
         tc_after();
         out(count - 1, last_win, 0.f);
       }
+      if (__any_sync(0xffffffffu, *odd_seen))
+        tc_spoil<DOTS, WIDE>(p, p.dots + (((int64_t)slice * 2 + part) * BH + bh) * a.T * 2, b, h, c0, count, len, row, n0 + 32 * part,
+                             first_row, row_step);
       // behind the sequence: zeros
       if (p.o) {
         const int64_t begin = (int64_t)(c0 + count) * C, stop = min(a.T, (int64_t)c1 * C);
@@ -747,8 +760,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
           }
         }
         unsigned char* const zw = tc_smem + L.zw + row * 128;
-        const TcPair wt2(wt, wt), zero2(0.f, 0.f);
-        TcPair odd(0.f, 0.f);   // stays zero unless a value is infinite or NaN
+        const TcPair wt2(wt, wt);
+        __nv_bfloat162 most = __floats2bfloat162_rn(0.f, 0.f);   // largest magnitudes: infinite or NaN where a value is
 #pragma unroll 1
         for (int q = 4 * part; q < 4 * part + 4; ++q) {
           const int at = (q ^ (row & 7)) << 4;
@@ -758,9 +771,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
           TcPair v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = tc_widen(in[e]);
-            if (!STATES_ONLY) odd = fma2(v[e], zero2, odd);
-            v[e] = v[e] * wt2;
+            v[e] = tc_widen(in[e]) * wt2;
+            if (!STATES_ONLY) most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&in[e])));
             t[e] = tc_pack(v[e]);
           }
           *reinterpret_cast<uint4*>(zw + at) = make_uint4(t[0], t[1], t[2], t[3]);
@@ -777,10 +789,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) la_tc_kernel(const __grid_const
           }
         }
         if constexpr (!STATES_ONLY) {
-          const float2 f = odd.get();
-          if (!(f.x + f.y == 0.f)) {
+          if (!(__low2float(most) < INFINITY && __high2float(most) < INFINITY)) {
             tc_take_out(tc_smem + zoff, row, part);
-            odd_chunk[i & 3] = i + 1;
+            *odd_seen = 1;
           }
         }
       }
