@@ -234,9 +234,9 @@ def _linear_attention_step(q, k, v, log_decay, state, scale, wide=False):
     o = (state if wide else v).new_empty((B, H, Dv))   # wide: in the sums' type, for a normalisation that follows
     if B and H:
         gs = _array((0, log_decay.stride(0)) if log_decay.dim() == 1 else log_decay.stride())
-        _lib.launch(lib.ptb_linear_attention_step_sums if wide else lib.ptb_linear_attention_step, dev, _code(q), B, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k),
-                    _outer_strides(k), ptr(v), _outer_strides(v), ptr(log_decay), gs, scale, ptr(state),
-                    _array(state.stride()[:2]), ptr(o))
+        entry = lib.ptb_linear_attention_step_sums if wide else lib.ptb_linear_attention_step
+        _lib.launch(entry, dev, _code(q), B, H, Dk, Dv, ptr(q), _outer_strides(q), ptr(k), _outer_strides(k), ptr(v), _outer_strides(v),
+                    ptr(log_decay), gs, scale, ptr(state), _array(state.stride()[:2]), ptr(o))
         torch.autograd.graph.increment_version(state)
     return o
 
